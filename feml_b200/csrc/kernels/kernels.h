@@ -225,6 +225,46 @@ int launch_silu_f32(const void *x, const uint64_t *xnb, void *y, const uint64_t 
                     cudaStream_t s);
 int launch_bias_act(void *y, uint64_t y_nb1, int64_t M, int64_t N, const EpiAct &epi, cudaStream_t s);
 
+// ---- e4m3 operators (f8.cuh: values, scales) --------------------------------
+// Where a row operator writes: q row r at q + r*q_nb1 (one byte per value),
+// its scales (one f32 per 128 values, or per 128 x 128 block) at scale +
+// r*scale_nb1.
+struct F8Out {
+    void *q;
+    uint64_t q_nb1;
+    float *scale;
+    uint64_t scale_nb1;
+};
+// quantize_f8.cu: rows of x (or silu(x) * up when `up` is given); x in type
+// FB_F32, FB_F16 or FB_BF16.
+int launch_rows_f8(int32_t type, const void *x, uint64_t x_nb1, const void *up, uint64_t up_nb1, int64_t rows,
+                   int64_t k, const F8Out &o, cudaStream_t s);
+int launch_quantize_f8_tiles(int32_t type, const void *x, uint64_t x_nb1, int64_t rows, int64_t k, const F8Out &o,
+                             cudaStream_t s);
+int launch_rms_norm_f8(int32_t type, const void *x, uint64_t x_nb1, const void *residual, uint64_t residual_nb1,
+                       void *sum, uint64_t sum_nb1, int32_t wtype, const void *weight, float eps, int64_t rows,
+                       int64_t k, const F8Out &o, cudaStream_t s);
+
+// Row groups of a grouped product (device tables; counts == null: ungrouped).
+struct F8Groups {
+    const int32_t *counts, *offsets, *rows;
+    int n_experts, n_rows, n_selected, n_x;
+};
+// Operands of an e4m3 product: N output rows (grouped: the rows of the
+// output buffer), weight rows at w + e*w_nb2 + m*w_nb1.
+struct F8Gemm {
+    const uint8_t *w, *ws, *x, *xs;
+    uint64_t w_nb1, w_nb2, ws_nb1, ws_nb2, x_nb1, xs_nb1;
+    uint8_t *y;
+    uint64_t y_nb1;
+    int32_t out_type;
+    int K, M, N;
+    F8Groups g;
+    int32_t *status;
+};
+// gemm_f8_any.cu: any alignment.
+int launch_gemm_f8_any(const F8Gemm &p, cudaStream_t s);
+
 int sm_count();
 
 }  // namespace fbk

@@ -1,0 +1,531 @@
+// Row operators that end in the e4m3 form (f8.cuh): plain quantization of
+// activations, silu(gate) * up, rms_norm with the residual's addition, and
+// the quantization of a weight matrix in 128 x 128 blocks.
+//
+// All of them are bound by memory: a few operations per byte, every value
+// read once and written once. The block maximum is taken of values that stay
+// in registers between the load and the store, so no operator makes a second
+// pass over its input.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "../host_common.h"
+#include "f8.cuh"
+#include "kernels.h"
+
+namespace fbk {
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// quantize (one operand) and silu_mul (two): blocks are independent. A block
+// of 128 values belongs to G consecutive lanes that hold one 16-byte vector
+// each (G = 16 for 16-bit types, 32 for f32); its maximum is a shuffle
+// reduction over them. Where rows or pointers are not 16-byte aligned a warp
+// takes a block with single-element accesses, lane l elements l, l + 32, ...
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 256;
+
+struct RowParams {
+    const uint8_t *x, *y;  // y: up (silu_mul)
+    uint64_t x_nb1, y_nb1;
+    uint8_t *q;
+    uint64_t q_nb1;
+    uint8_t *s;
+    uint64_t s_nb1;
+    int64_t total;  // rows * blocks per row
+    int64_t k;
+    uint32_t kb;    // blocks per row
+};
+
+// silu(g) * u = g / (1 + e^-g) * u. The exponential and the division are the
+// fast forms (a few units in the last place of f32; the result goes to 4
+// significant bits): with the exact ones the kernel is bound by arithmetic
+// instead of memory.
+__device__ __forceinline__ float silu_mul_f(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+template <typename T, bool SILU, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) rows_f8_kernel(const RowParams p) {
+    constexpr int N = VEC ? Vec<T>::N : 4;
+    constexpr int G = F8B / N;
+    const int lane = threadIdx.x % G;
+    const int64_t gid = (int64_t)blockIdx.x * (kRowThreads / G) + threadIdx.x / G;
+    const bool live = gid < p.total;
+    // one division by the blocks per row, in 32 bits where the count allows
+    int64_t row;
+    uint32_t b;
+    if (p.total <= 0x7fffffff) {
+        row = (uint32_t)gid / p.kb;
+        b = (uint32_t)gid - (uint32_t)row * p.kb;
+    } else {
+        row = gid / p.kb;
+        b = (uint32_t)(gid - row * p.kb);
+    }
+    const int64_t k0 = (int64_t)b * F8B;
+    const uint8_t *xr = p.x + row * p.x_nb1;
+    const uint8_t *yr = SILU ? p.y + row * p.y_nb1 : nullptr;
+    float f[N];
+    uint32_t top = 0;
+    if constexpr (VEC) {
+        const int64_t k = k0 + lane * N;  // k % N == 0 here: a vector lies inside the row or outside
+        const bool in = live && k < p.k;
+        uint4 v = make_uint4(0, 0, 0, 0), w = v;
+        if (in) {
+            v = ld_stream16(xr + k * sizeof(T));
+            if constexpr (SILU) w = ld_stream16(yr + k * sizeof(T));
+        }
+        Vec<T>::get(v, f);
+        if constexpr (SILU) {
+            float u[N];
+            Vec<T>::get(w, u);
+#pragma unroll
+            for (int i = 0; i < N; i++) f[i] = silu_mul_f(f[i], u[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int64_t k = k0 + lane + i * 32;
+            f[i] = 0.0f;
+            if (live && k < p.k) {
+                f[i] = to_f32(reinterpret_cast<const T *>(xr)[k]);
+                if constexpr (SILU) f[i] = silu_mul_f(f[i], to_f32(reinterpret_cast<const T *>(yr)[k]));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) top = max(top, abs_bits(f[i]));
+#pragma unroll
+    for (int o = 1; o < G; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float s, r;
+    f8_scale(top, s, r);
+    if (!live) return;
+    uint8_t *qr = p.q + row * p.q_nb1;
+    if constexpr (VEC) {
+        const int64_t k = k0 + lane * N;
+        if (k < p.k) {
+            const uint32_t lo = f8_pack4(f[0] * r, f[1] * r, f[2] * r, f[3] * r);
+            if constexpr (N == 8) {
+                const uint32_t hi = f8_pack4(f[4] * r, f[5] * r, f[6] * r, f[7] * r);
+                *reinterpret_cast<uint2 *>(qr + k) = make_uint2(lo, hi);
+            } else {
+                *reinterpret_cast<uint32_t *>(qr + k) = lo;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int64_t k = k0 + lane + i * 32;
+            if (k < p.k) qr[k] = f8_one(f[i] * r);
+        }
+    }
+    if (lane == 0) reinterpret_cast<float *>(p.s + row * p.s_nb1)[b] = s;
+}
+
+// ---------------------------------------------------------------------------
+// Weights: one CTA per 128 x 128 block, its values in registers.
+// ---------------------------------------------------------------------------
+constexpr int kTileThreads = 512;
+
+struct TileParams {
+    const uint8_t *x;
+    uint64_t x_nb1;
+    uint8_t *q;
+    uint64_t q_nb1;
+    uint8_t *s;
+    uint64_t s_nb1;
+    int64_t rows, k;
+    uint32_t kb;
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kTileThreads) tile_f8_kernel(const TileParams p) {
+    constexpr int N = VEC ? Vec<T>::N : 1;
+    constexpr int G = F8B / N;                  // threads per row
+    constexpr int RS = kTileThreads / G;        // rows per step
+    constexpr int STEPS = F8B / RS;
+    __shared__ uint32_t s_top[kTileThreads / 32];
+    const int64_t br = blockIdx.x / p.kb;
+    const uint32_t bc = (uint32_t)(blockIdx.x - br * p.kb);
+    const int64_t k = (int64_t)bc * F8B + (threadIdx.x % G) * N;
+    const int64_t row0 = br * F8B + threadIdx.x / G;
+    const bool in_k = k < p.k;
+    uint4 v[VEC ? STEPS : 1];
+    float e[VEC ? 1 : STEPS];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        const int64_t row = row0 + i * RS;
+        const bool in = in_k && row < p.rows;
+        const uint8_t *a = p.x + row * p.x_nb1 + k * sizeof(T);
+        if constexpr (VEC)
+            v[i] = in ? ld_stream16(a) : make_uint4(0, 0, 0, 0);
+        else
+            e[i] = in ? to_f32(*reinterpret_cast<const T *>(a)) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        if constexpr (VEC) {
+            float f[N];
+            Vec<T>::get(v[i], f);
+#pragma unroll
+            for (int j = 0; j < N; j++) top = max(top, abs_bits(f[j]));
+        } else {
+            top = max(top, abs_bits(e[i]));
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, s_top[threadIdx.x % (kTileThreads / 32)]);
+    float s, r;
+    f8_scale(top, s, r);
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        const int64_t row = row0 + i * RS;
+        if (!in_k || row >= p.rows) continue;
+        uint8_t *q = p.q + row * p.q_nb1 + k;
+        if constexpr (VEC) {
+            float f[N];
+            Vec<T>::get(v[i], f);
+            const uint32_t lo = f8_pack4(f[0] * r, f[1] * r, f[2] * r, f[3] * r);
+            if constexpr (N == 8) {
+                const uint32_t hi = f8_pack4(f[4] * r, f[5] * r, f[6] * r, f[7] * r);
+                *reinterpret_cast<uint2 *>(q) = make_uint2(lo, hi);
+            } else {
+                *reinterpret_cast<uint32_t *>(q) = lo;
+            }
+        } else {
+            *q = f8_one(e[i] * r);
+        }
+    }
+    if (threadIdx.x == 0) reinterpret_cast<float *>(p.s + br * p.s_nb1)[bc] = s;
+}
+
+// ---------------------------------------------------------------------------
+// rms_norm: h = round(x + residual) is stored and kept in registers as it is
+// stored (so the fused call gives the bits of an addition followed by the
+// norm), y = (h * (1 / sqrt(mean(h^2) + eps))) * weight goes to the 8-bit
+// form. The sum of squares is held in f32 in a fixed order.
+// ---------------------------------------------------------------------------
+struct NormF8Params {
+    const uint8_t *x, *res, *w;
+    uint64_t x_nb1, res_nb1;
+    uint8_t *sum;
+    uint64_t sum_nb1;
+    uint8_t *q;
+    uint64_t q_nb1;
+    uint8_t *s;
+    uint64_t s_nb1;
+    int64_t rows, k;
+    float eps;
+    int w_f32;  // weight in f32 (else in the type of x)
+};
+
+// Sum over the CTA's warps, in warp order; the same value in every thread.
+__device__ __forceinline__ float cta_sum(float v, float *part) {
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
+    return warp_sum(lane < nw ? part[lane] : 0.0f);
+}
+
+// The row in registers: NV vectors per thread. WARP: a warp per row
+// (blockDim.y rows per CTA), else a CTA per row.
+template <typename T, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8Params p) {
+    constexpr int N = Vec<T>::N, G = F8B / N;
+    __shared__ float part[32];
+    const int64_t row = WARP ? (int64_t)blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
+    if (WARP && row >= p.rows) return;
+    const int t = threadIdx.x, nt = WARP ? 32 : blockDim.x;
+    const uint8_t *xr = p.x + row * p.x_nb1;
+    uint4 v[NV];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int64_t k = (int64_t)(i * nt + t) * N;
+        v[i] = k < p.k ? ld_stream16(xr + k * sizeof(T)) : make_uint4(0, 0, 0, 0);
+    }
+    if (p.res) {
+        const uint8_t *rr = p.res + row * p.res_nb1;
+        uint8_t *hr = p.sum + row * p.sum_nb1;
+        uint4 u[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int64_t k = (int64_t)(i * nt + t) * N;
+            u[i] = k < p.k ? ld_stream16(rr + k * sizeof(T)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int64_t k = (int64_t)(i * nt + t) * N;
+            float a[N], b[N];
+            Vec<T>::get(v[i], a);
+            Vec<T>::get(u[i], b);
+#pragma unroll
+            for (int j = 0; j < N; j++) a[j] += b[j];
+            v[i] = Vec<T>::put(a);
+            if (k < p.k) *reinterpret_cast<uint4 *>(hr + k * sizeof(T)) = v[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        float f[N];
+        Vec<T>::get(v[i], f);
+#pragma unroll
+        for (int j = 0; j < N; j++) ss = fmaf(f[j], f[j], ss);
+    }
+    ss = WARP ? warp_sum(ss) : cta_sum(ss, part);
+    const float inv = 1.0f / sqrtf(ss / (float)p.k + p.eps);
+    uint8_t *qr = p.q + row * p.q_nb1;
+    float *sr = reinterpret_cast<float *>(p.s + row * p.s_nb1);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int64_t k = (int64_t)(i * nt + t) * N;
+        const bool in = k < p.k;
+        float f[N];
+        Vec<T>::get(v[i], f);
+        uint32_t top = 0;
+        if (in) {
+            float g[N];
+            if (sizeof(T) == 4 || !p.w_f32) {
+                Vec<T>::get(__ldg(reinterpret_cast<const uint4 *>(p.w + k * sizeof(T))), g);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j += 4) {
+                    const float4 w4 = __ldg(reinterpret_cast<const float4 *>(p.w + (k + j) * 4));
+                    g[j] = w4.x;
+                    g[j + 1] = w4.y;
+                    g[j + 2] = w4.z;
+                    g[j + 3] = w4.w;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                f[j] = f[j] * inv * g[j];
+                top = max(top, abs_bits(f[j]));
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float s, r;
+        f8_scale(top, s, r);
+        if (in) {
+            const uint32_t lo = f8_pack4(f[0] * r, f[1] * r, f[2] * r, f[3] * r);
+            if constexpr (N == 8) {
+                const uint32_t hi = f8_pack4(f[4] * r, f[5] * r, f[6] * r, f[7] * r);
+                *reinterpret_cast<uint2 *>(qr + k) = make_uint2(lo, hi);
+            } else {
+                *reinterpret_cast<uint32_t *>(qr + k) = lo;
+            }
+            if (t % G == 0) sr[k / F8B] = s;
+        }
+    }
+}
+
+// Rows of any length and alignment: the sum of squares in one pass, the norm
+// in a second one that reads the stored sum (or x) again, a warp per block.
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_f8_any_kernel(const NormF8Params p) {
+    __shared__ float part[32];
+    const int64_t row = blockIdx.x;
+    const T *x = reinterpret_cast<const T *>(p.x + row * p.x_nb1);
+    const T *res = p.res ? reinterpret_cast<const T *>(p.res + row * p.res_nb1) : nullptr;
+    T *sum = p.res ? reinterpret_cast<T *>(p.sum + row * p.sum_nb1) : nullptr;
+    float ss = 0.0f;
+    for (int64_t k = threadIdx.x; k < p.k; k += blockDim.x) {
+        float f = to_f32(x[k]);
+        if (res) {
+            const T h = from_f32<T>(f + to_f32(res[k]));
+            sum[k] = h;
+            f = to_f32(h);
+        }
+        ss = fmaf(f, f, ss);
+    }
+    ss = cta_sum(ss, part);  // its barrier also orders the stored sums before the reads below
+    const float inv = 1.0f / sqrtf(ss / (float)p.k + p.eps);
+    const T *h = res ? sum : x;
+    const int lane = threadIdx.x & 31;
+    uint8_t *qr = p.q + row * p.q_nb1;
+    float *sr = reinterpret_cast<float *>(p.s + row * p.s_nb1);
+    for (int64_t b = threadIdx.x >> 5; b * F8B < p.k; b += blockDim.x >> 5) {
+        float f[4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t k = b * F8B + lane + i * 32;
+            f[i] = 0.0f;
+            if (k < p.k) {
+                const float g = p.w_f32 ? reinterpret_cast<const float *>(p.w)[k] : to_f32(reinterpret_cast<const T *>(p.w)[k]);
+                f[i] = to_f32(h[k]) * inv * g;
+            }
+            top = max(top, abs_bits(f[i]));
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        float s, r;
+        f8_scale(top, s, r);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t k = b * F8B + lane + i * 32;
+            if (k < p.k) qr[k] = f8_one(f[i] * r);
+        }
+        if (lane == 0) sr[b] = s;
+    }
+}
+
+int launched(const char *what) {
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return fb::set_error(FB_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+    return FB_OK;
+}
+
+bool aligned(uint64_t a, const void *p, uint64_t nb1) { return ((reinterpret_cast<uintptr_t>(p) | nb1) & (a - 1)) == 0; }
+
+template <typename T, bool SILU>
+int launch_rows_t(const RowParams &p, bool vec, cudaStream_t s, const char *what) {
+    const int groups = kRowThreads / (vec ? F8B / Vec<T>::N : 32);
+    const int64_t grid = (p.total + groups - 1) / groups;
+    if (grid > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "%s: too many blocks", what);
+    if (vec)
+        rows_f8_kernel<T, SILU, true><<<(unsigned)grid, kRowThreads, 0, s>>>(p);
+    else
+        rows_f8_kernel<T, SILU, false><<<(unsigned)grid, kRowThreads, 0, s>>>(p);
+    return launched(what);
+}
+
+template <typename T>
+int launch_norm_t(const NormF8Params &p, bool vec, cudaStream_t s) {
+    constexpr int N = Vec<T>::N;
+    const int64_t vecs = p.k / N;
+    if (!vec || vecs > 8 * 1024) {
+        const int threads = (int)std::min<int64_t>(1024, (p.k + 31) / 32 * 32);
+        norm_f8_any_kernel<T><<<(unsigned)p.rows, threads, 0, s>>>(p);
+        return launched("rms_norm_f8");
+    }
+    // A warp per row for short rows in numbers that fill the GPU; else a CTA
+    // per row: one vector per thread when rows are few (latency), more
+    // vectors and small CTAs when they are many.
+    if (vecs <= 128 && p.rows >= 1024) {
+        const dim3 block(32, 8);
+        const unsigned grid = (unsigned)((p.rows + 7) / 8);
+        if (vecs <= 32)
+            norm_f8_kernel<T, 1, true><<<grid, block, 0, s>>>(p);
+        else if (vecs <= 64)
+            norm_f8_kernel<T, 2, true><<<grid, block, 0, s>>>(p);
+        else
+            norm_f8_kernel<T, 4, true><<<grid, block, 0, s>>>(p);
+        return launched("rms_norm_f8");
+    }
+    const int most = p.rows <= 296 ? 1024 : 256;
+    int nv = 1;
+    while (nv < 8 && (vecs + nv - 1) / nv > most) nv *= 2;
+    const int threads = (int)(((vecs + nv - 1) / nv + 31) / 32 * 32);
+    const unsigned grid = (unsigned)p.rows;
+    if (nv == 1)
+        norm_f8_kernel<T, 1, false><<<grid, threads, 0, s>>>(p);
+    else if (nv == 2)
+        norm_f8_kernel<T, 2, false><<<grid, threads, 0, s>>>(p);
+    else if (nv == 4)
+        norm_f8_kernel<T, 4, false><<<grid, threads, 0, s>>>(p);
+    else
+        norm_f8_kernel<T, 8, false><<<grid, threads, 0, s>>>(p);
+    return launched("rms_norm_f8");
+}
+
+int esize(int32_t type) { return type == FB_F32 ? 4 : 2; }
+
+}  // namespace
+
+int launch_rows_f8(int32_t type, const void *x, uint64_t x_nb1, const void *up, uint64_t up_nb1, int64_t rows,
+                   int64_t k, const F8Out &o, cudaStream_t s) {
+    const char *what = up ? "silu_mul_f8" : "quantize_f8";
+    RowParams p{};
+    p.x = static_cast<const uint8_t *>(x);
+    p.x_nb1 = x_nb1;
+    p.y = static_cast<const uint8_t *>(up);
+    p.y_nb1 = up_nb1;
+    p.q = static_cast<uint8_t *>(o.q);
+    p.q_nb1 = o.q_nb1;
+    p.s = reinterpret_cast<uint8_t *>(o.scale);
+    p.s_nb1 = o.scale_nb1;
+    p.k = k;
+    p.kb = (uint32_t)((k + F8B - 1) / F8B);
+    p.total = rows * p.kb;
+    const int n = 16 / esize(type);
+    const bool vec = k % n == 0 && aligned(16, x, x_nb1) && (!up || aligned(16, up, up_nb1)) && aligned(n, o.q, o.q_nb1);
+    switch (type) {
+        case FB_F32:
+            return up ? launch_rows_t<float, true>(p, vec, s, what) : launch_rows_t<float, false>(p, vec, s, what);
+        case FB_F16:
+            return up ? launch_rows_t<__half, true>(p, vec, s, what) : launch_rows_t<__half, false>(p, vec, s, what);
+        default:
+            return up ? launch_rows_t<__nv_bfloat16, true>(p, vec, s, what)
+                      : launch_rows_t<__nv_bfloat16, false>(p, vec, s, what);
+    }
+}
+
+int launch_quantize_f8_tiles(int32_t type, const void *x, uint64_t x_nb1, int64_t rows, int64_t k, const F8Out &o,
+                             cudaStream_t s) {
+    TileParams p{};
+    p.x = static_cast<const uint8_t *>(x);
+    p.x_nb1 = x_nb1;
+    p.q = static_cast<uint8_t *>(o.q);
+    p.q_nb1 = o.q_nb1;
+    p.s = reinterpret_cast<uint8_t *>(o.scale);
+    p.s_nb1 = o.scale_nb1;
+    p.rows = rows;
+    p.k = k;
+    p.kb = (uint32_t)((k + F8B - 1) / F8B);
+    const int64_t grid = (rows + F8B - 1) / F8B * p.kb;
+    if (grid > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "quantize_f8: too many blocks");
+    const int n = 16 / esize(type);
+    const bool vec = k % n == 0 && aligned(16, x, x_nb1) && aligned(n, o.q, o.q_nb1);
+    const unsigned g = (unsigned)grid;
+#define FB_TILE(T)                                            \
+    if (vec)                                                  \
+        tile_f8_kernel<T, true><<<g, kTileThreads, 0, s>>>(p); \
+    else                                                      \
+        tile_f8_kernel<T, false><<<g, kTileThreads, 0, s>>>(p);
+    if (type == FB_F32) {
+        FB_TILE(float)
+    } else if (type == FB_F16) {
+        FB_TILE(__half)
+    } else {
+        FB_TILE(__nv_bfloat16)
+    }
+#undef FB_TILE
+    return launched("quantize_f8");
+}
+
+int launch_rms_norm_f8(int32_t type, const void *x, uint64_t x_nb1, const void *residual, uint64_t residual_nb1,
+                       void *sum, uint64_t sum_nb1, int32_t wtype, const void *weight, float eps, int64_t rows,
+                       int64_t k, const F8Out &o, cudaStream_t s) {
+    NormF8Params p{};
+    p.x = static_cast<const uint8_t *>(x);
+    p.x_nb1 = x_nb1;
+    p.res = static_cast<const uint8_t *>(residual);
+    p.res_nb1 = residual_nb1;
+    p.sum = static_cast<uint8_t *>(sum);
+    p.sum_nb1 = sum_nb1;
+    p.w = static_cast<const uint8_t *>(weight);
+    p.w_f32 = wtype == FB_F32;
+    p.q = static_cast<uint8_t *>(o.q);
+    p.q_nb1 = o.q_nb1;
+    p.s = reinterpret_cast<uint8_t *>(o.scale);
+    p.s_nb1 = o.scale_nb1;
+    p.rows = rows;
+    p.k = k;
+    p.eps = eps;
+    const int n = 16 / esize(type);
+    const bool vec = k % n == 0 && aligned(16, x, x_nb1) && aligned(16, weight, 0) &&
+                     (!residual || (aligned(16, residual, residual_nb1) && aligned(16, sum, sum_nb1))) &&
+                     aligned(n, o.q, o.q_nb1);
+    switch (type) {
+        case FB_F32: return launch_norm_t<float>(p, vec, s);
+        case FB_F16: return launch_norm_t<__half>(p, vec, s);
+        default: return launch_norm_t<__nv_bfloat16>(p, vec, s);
+    }
+}
+
+}  // namespace fbk

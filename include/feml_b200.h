@@ -480,6 +480,77 @@ int feml_b200_moe_route(const int32_t *ids, uint64_t ids_nb1, int64_t n_selected
 int feml_b200_block_dots(int32_t wtype, const void *w, uint64_t w_nb1, const void *xq, int64_t K, int64_t M,
                          int64_t N, int32_t *out, void *stream);
 
+/* ---- e4m3 operators: 8-bit floating point with block scales ---------------- */
+
+/* The 8-bit form of a matrix: e4m3 values q (one byte each) with one f32
+ * scale per 128 consecutive values of a row (activations), or per block of
+ * 128 x 128 values (weights); blocks at the edges are smaller. A value is
+ * q * scale. A block with largest magnitude a gets, with a' = max(a, 2^-100),
+ *   scale = a' / 448,   q = e4m3(y * (448 / a')), rounded to nearest even;
+ * a block that holds an infinity or a NaN gets NaN for its scale and every q.
+ * The reference has no 8-bit floating point type: the ids below belong to
+ * these calls alone (they are ggml's). Types of x, sums and dst are FB_F32,
+ * FB_F16 or FB_BF16. Rows are contiguous, their strides (nb1, bytes) any
+ * multiple of the element size that keeps rows apart. Sums, norms and
+ * products are held in f32; dst is rounded once, to nearest even. Empty
+ * operands (no rows, k = 0) are no error. Outputs must not overlap inputs,
+ * except where said. */
+#define FB_BF16 30
+
+/* rows x k values of x into the 8-bit form: q row r at q + r*q_nb1, and with
+ * block_rows = 1 (activations) its ceil(k/128) scales at scale +
+ * r*scale_nb1, with block_rows = 128 (weights) the scales of block row i at
+ * scale + i*scale_nb1. */
+int feml_b200_quantize_f8(int32_t xtype, const void *x, uint64_t x_nb1, int64_t rows, int64_t k, int64_t block_rows,
+                          void *q, uint64_t q_nb1, float *scale, uint64_t scale_nb1, void *stream);
+
+/* rms_norm with the residual's addition, into the 8-bit form:
+ *   h = x + residual, rounded to the type of x and stored to sum
+ *   y = h * (1 / sqrt(mean_k(h^2) + eps)) * weight  -> q, scale (per row)
+ * The norm is that of the stored sum, so the call gives the bits of an
+ * addition followed by the norm. residual == NULL: h = x and sum is not
+ * written. sum may be x or residual itself (exactly, same stride). weight: k
+ * values of type wtype, the type of x or FB_F32. Relative of
+ * feml_b200_graph_compute's rms_norm (feml-core/src/op.rs:26). */
+int feml_b200_rms_norm_f8(int32_t xtype, const void *x, uint64_t x_nb1, const void *residual, uint64_t residual_nb1,
+                          void *sum, uint64_t sum_nb1, int32_t wtype, const void *weight, float eps, int64_t rows,
+                          int64_t k, void *q, uint64_t q_nb1, float *scale, uint64_t scale_nb1, void *stream);
+
+/* y = gate / (1 + exp(-gate)) * up, into the 8-bit form (per row). gate and
+ * up may be the halves of one matrix. */
+int feml_b200_silu_mul_f8(int32_t xtype, const void *gate, uint64_t gate_nb1, const void *up, uint64_t up_nb1,
+                          int64_t rows, int64_t k, void *q, uint64_t q_nb1, float *scale, uint64_t scale_nb1,
+                          void *stream);
+
+/* mul_mat on the 8-bit form, ggml layout (dst row n = output column n):
+ *   dst[n][m] = sum_b xs[n][b] * ws[m/128][b] * (sum_{k in b} x[n][k] * w[m][k])
+ * w: e4m3, row m at w + m*w_nb1; w_scale: block row i at w_scale +
+ * i*w_scale_nb1; x: e4m3, row n at x + n*x_nb1; x_scale row n at x_scale +
+ * n*x_scale_nb1; dst row n at dst + n*dst_nb1. 16-byte aligned w and x with
+ * strides that are multiples of 16 take the TMA kernels; any other alignment
+ * works and is slower. No workspace, no allocation. */
+int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, uint64_t w_scale_nb1, const void *x,
+                         uint64_t x_nb1, const float *x_scale, uint64_t x_scale_nb1, int32_t dst_type, void *dst,
+                         uint64_t dst_nb1, int64_t K, int64_t M, int64_t N, void *stream);
+
+/* The same product for rows grouped by expert (ragged groups, known on the
+ * device only): rows offsets[e] .. offsets[e] + counts[e] - 1 of dst are
+ * multiplied with expert e's weights (w + e*w_nb2, w_scale + e*w_scale_nb2).
+ * Row r of dst takes row rows[r] / n_selected of x, or row r when rows is
+ * NULL: counts, offsets and rows are feml_b200_moe_route's tables, with
+ * n_selected experts per token for a product that reads the tokens, and 1
+ * for one that reads slots. x has n_x rows, dst (and rows) n_rows; groups
+ * must not overlap, and rows of dst in no group are left as they were.
+ * A group that does not lie inside [0, n_rows) is skipped and a row of dst
+ * whose source lies outside x becomes zeros; both set bit 1 of *status
+ * (device int32, may be NULL). At most 1024 experts. */
+int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, const float *w_scale,
+                                 uint64_t w_scale_nb1, uint64_t w_scale_nb2, int64_t n_experts, const void *x,
+                                 uint64_t x_nb1, int64_t n_x, const float *x_scale, uint64_t x_scale_nb1,
+                                 const int32_t *counts, const int32_t *offsets, const int32_t *rows,
+                                 int64_t n_selected, int32_t dst_type, void *dst, uint64_t dst_nb1, int64_t K,
+                                 int64_t M, int64_t n_rows, int32_t *status, void *stream);
+
 /* ---- weight ingestion: host pointers and GGUF files ----------------------- */
 
 /* BackendDevice::buffer_from_host_ptr (feml-core/src/backend.rs:145-153; the
