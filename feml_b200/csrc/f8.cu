@@ -57,9 +57,8 @@ int check_out(const char *op, const fbk::F8Out &o, int64_t rows, int64_t k, int6
 // A row stride that no second row uses must not decide alignment.
 uint64_t stride_of(uint64_t nb1, int64_t rows, int64_t bytes) { return rows > 1 ? nb1 : (uint64_t)(bytes + 15) / 16 * 16; }
 
-int run_product(const char *op, fbk::F8Gemm &p, int64_t n_experts, cudaStream_t s) {
-    (void)op;
-    (void)n_experts;
+int run_product(const fbk::F8Gemm &p, cudaStream_t s) {
+    if (fbk::gemm_f8_supported(p)) return fbk::launch_gemm_f8(p, s);
     return fbk::launch_gemm_f8_any(p, s);
 }
 
@@ -161,7 +160,7 @@ int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, ui
     p.K = (int)K;
     p.M = (int)M;
     p.N = (int)N;
-    return run_product(op, p, 0, s);
+    return run_product(p, s);
 }
 
 int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, const float *w_scale,
@@ -220,7 +219,7 @@ int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, 
     p.g.n_selected = (int)n_selected;
     p.g.n_x = (int)n_x;
     p.status = status;
-    return run_product(op, p, n_experts, static_cast<cudaStream_t>(stream));
+    return run_product(p, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,526 @@
+// e4m3 matrix product on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
+//
+// Mathematics: gemm_f8.cuh. The f32 scales of a block of 128 cannot enter the
+// tensor core, so every block's product is a fresh accumulation in TMEM (four
+// kind::f8f6f4 MMAs of K = 32) that the epilogue warps read, scale and add to
+// f32 registers. The activations are the MMA's M side: a thread of the
+// epilogue then owns one row (one TMEM lane), its block scale is one scalar
+// xs[row][b] * ws[m block][b], and the promotion is one packed FMA per two
+// values.
+//
+// Roles of a CTA of 384 threads, one per SM, persistent over tiles of 128
+// rows x BN weight rows:
+//   warp 0      TMA producer: 128 x 128 bytes of x and BN x 128 bytes of w per
+//               stage (128-byte swizzle); gathered rows with tile::gather4
+//   warp 1      issues the MMAs of a block into one of 512 / BN TMEM buffers
+//   warp 2      allocates TMEM
+//   warps 4-11  promote: two warpgroups, BN / 2 columns each; at a tile's end
+//               they round, transpose through shared memory and store rows
+// A 128 x 256 tile needs 512 cycles of MMA per block; reading its 32768
+// accumulators takes 256 cycles of TMEM bandwidth and the FMAs 128 issue
+// slots per warp, so promotion hides behind the MMAs of the next block.
+//
+// SPLIT: few tiles. A cluster of S CTAs shares a tile, each takes a range of
+// blocks; the partial tiles meet in distributed shared memory and are added
+// in rank order, so no workspace is needed and the result does not depend on
+// timing.
+//
+// Every wait is bounded; when one runs out the CTA raises STATUS_TIMEOUT, lets
+// its copies and MMAs land, frees TMEM and returns.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "../host_common.h"
+#include "gemm_f8.cuh"
+#include "tc.cuh"
+#include "tmap.h"
+
+namespace fbk {
+
+namespace {
+
+constexpr int GM = 128;           // rows per tile
+constexpr int G_THREADS = 384;
+constexpr int G_EPI_WARPS = 8;
+constexpr int G_XBOX = 32;        // rows per TMA box of x: only boxes with live rows are fetched
+constexpr int G_MAX_E = 1024;
+constexpr int G_REGS_EPI = 216, G_REGS_REST = 40;
+
+template <int BN>
+struct GCfg {
+    static constexpr int X_STAGE = GM * F8B;
+    static constexpr int W_STAGE = BN * F8B;
+    static constexpr int STAGE = X_STAGE + W_STAGE;
+    static constexpr int NS = BN == 256 ? 4 : 6;  // stages
+    static constexpr int NB = 512 / BN;           // TMEM buffers
+    static constexpr int COLS = BN / 2;           // columns per epilogue warpgroup
+    static constexpr int OFF_OUT = NS * STAGE;    // 2 KB per epilogue warp
+    static constexpr int OFF_GRP = OFF_OUT + G_EPI_WARPS * 2048;
+    static constexpr int OFF_BAR = OFF_GRP + (G_MAX_E + 1) * 4 + 12;
+    static constexpr int BYTES = OFF_BAR + (2 * NS + 2 * NB + 1) * 8 + 16 + 1024;
+    static_assert(OFF_BAR % 8 == 0 && BYTES <= 232448, "shared memory");
+    static_assert(GM * (BN + 4) * 4 <= NS * STAGE, "partial tile of a split");
+};
+
+struct GParams {
+    F8Gemm p;
+    int tiles_m, tiles_n;  // tiles of weight rows; of rows (ungrouped)
+    int band;              // row tiles walked together (ungrouped)
+    int kb;                // blocks
+};
+
+struct GTile {
+    int expert, m0, row0, rows;
+};
+
+__device__ __forceinline__ void mma_f8f6f4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
+        : "memory");
+}
+
+// Instruction descriptor, kind::f8f6f4: D f32, A and B e4m3, both K-major.
+constexpr uint32_t f8_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+
+// Four rows (any four) of one 128-byte column box.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, int c0, int r0, int r1, int r2, int r3,
+                                            uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+        : "memory");
+}
+
+// Tile `t` (expert < 0 past the last). Ungrouped: bands of row tiles, all
+// weight tiles of a band before the next band, so that the CTAs running at a
+// time share both operands through L2. Grouped: `start` holds every group's
+// first tile; a weight tile's row tiles are neighbours.
+__device__ __forceinline__ GTile g_tile(const GParams &q, const int *start, int t, int bn) {
+    if (!q.p.g.counts) {
+        if (t >= q.tiles_m * q.tiles_n) return {-1, 0, 0, 0};
+        const int per = q.band * q.tiles_m, b = t / per, r = t - b * per;
+        const int wide = min(q.band, q.tiles_n - b * q.band);
+        const int row0 = (b * q.band + r % wide) * GM;
+        return {0, r / wide * bn, row0, min(GM, q.p.N - row0)};
+    }
+    const int E = q.p.g.n_experts;
+    if (t >= start[E]) return {-1, 0, 0, 0};
+    int lo = 0, hi = E;  // last group whose first tile is <= t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= t)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const F8Group g = f8_group(q.p.g, lo, nullptr);
+    const int nt = (g.rows + GM - 1) / GM, r = t - start[lo];
+    const int at = r % nt * GM;
+    return {lo, r / nt * bn, g.row0 + at, min(GM, g.rows - at)};
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float *f) {
+    float v[Vec<T>::N];
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; i++) v[i] = f[i];
+    return Vec<T>::put(v);
+}
+
+// 16 bytes of one output row; element by element where the row's end or the
+// alignment asks for it.
+template <typename T>
+__device__ __forceinline__ void store16(uint8_t *row, int m, int M, uint4 v, bool wide) {
+    T *o = reinterpret_cast<T *>(row) + m;
+    if (wide && m + Vec<T>::N <= M) {
+        *reinterpret_cast<uint4 *>(o) = v;
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; i++) {
+            if (m + i >= M) break;
+            if constexpr (sizeof(T) == 4)
+                o[i] = __uint_as_float(w[i]);
+            else
+                reinterpret_cast<uint16_t *>(o)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        }
+    }
+}
+
+// One warp's 32 rows x COLS columns of finished sums (a row per lane): 64
+// bytes of each row at a time through 2 KB of shared memory, so that the
+// global stores cover whole sectors. 16-byte unit u of row r lies at
+// u ^ ((r >> 1) & 3): neither side has bank conflicts.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_rows(const float (&acc)[COLS], uint32_t stage, const GTile &t, int r_first, int m0,
+                                           const F8Gemm &p, int lane, bool wide) {
+    constexpr int N = Vec<T>::N;
+#pragma unroll
+    for (int c = 0; c < COLS; c += 4 * N) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const uint4 v = pack16<T>(&acc[c + u * N]);
+            const uint32_t a = stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = i * 8 + (lane >> 2), u = lane & 3;
+            uint4 v;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(stage + r * 64 + ((u ^ ((r >> 1) & 3)) << 4))
+                         : "memory");
+            const int m = m0 + c + u * N;
+            if (r_first + r < t.rows && m < p.M)
+                store16<T>(p.y + (uint64_t)(t.row0 + r_first + r) * p.y_nb1, m, p.M, v, wide);
+        }
+        __syncwarp();
+    }
+}
+
+template <int BN, bool SPLIT, bool GATHER>
+__global__ void __launch_bounds__(G_THREADS, 1)
+    gemm_f8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                   const __grid_constant__ GParams q) {
+    using C = GCfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *gbase = smem_raw + (sbase - smem_u32(smem_raw));
+    int *start = reinterpret_cast<int *>(gbase + C::OFF_GRP);
+    uint64_t *full = reinterpret_cast<uint64_t *>(gbase + C::OFF_BAR);
+    uint64_t *empty = full + C::NS;
+    uint64_t *t_full = empty + C::NS;
+    uint64_t *t_empty = t_full + C::NB;
+    uint64_t *drained = t_empty + C::NB;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const F8Gemm &p = q.p;
+
+    if (tid == 0) {
+        for (int i = 0; i < C::NS; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < C::NB; i++) {
+            mbar_init(&t_full[i], 1);
+            mbar_init(&t_empty[i], G_EPI_WARPS);
+        }
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == 3 && p.g.counts) {  // first tile of every group
+        int run = 0;
+        for (int e0 = 0; e0 < p.g.n_experts; e0 += 32) {
+            int n = 0;
+            if (e0 + lane < p.g.n_experts)
+                n = (f8_group(p.g, e0 + lane, blockIdx.x == 0 ? p.status : nullptr).rows + GM - 1) / GM * q.tiles_m;
+            int sum = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            if (e0 + lane < p.g.n_experts) start[e0 + lane] = run + sum - n;
+            run += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) start[p.g.n_experts] = run;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int S = SPLIT ? (int)cluster_size() : 1, rank = SPLIT ? (int)cluster_rank() : 0;
+    const int t0 = (int)blockIdx.x / S, t_step = SPLIT ? 0x40000000 : (int)gridDim.x;
+    const int b0 = SPLIT ? (int)((int64_t)q.kb * rank / S) : 0, b1 = SPLIT ? (int)((int64_t)q.kb * (rank + 1) / S) : q.kb;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G_REGS_REST));
+        if (warp == 0) {
+            // ---- TMA producer ---------------------------------------------------
+            int it = 0;
+            bool ok = true;
+            for (int t = t0; ok; t += t_step) {
+                const GTile tile = g_tile(q, start, t, BN);
+                if (tile.expert < 0) break;
+                int r[4] = {0, 0, 0, 0};
+                if constexpr (GATHER) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (lane * 4 + j < tile.rows) r[j] = max(0, f8_source(p.g, tile.row0 + lane * 4 + j, nullptr));
+                }
+                const int boxes = (tile.rows + G_XBOX - 1) / G_XBOX, quads = (tile.rows + 3) / 4;
+                const uint32_t bytes = C::W_STAGE + (GATHER ? quads * 4 * F8B : boxes * G_XBOX * F8B);
+                for (int b = b0; b < b1; b++, it++) {
+                    const int s = it % C::NS;
+                    if (!tc_wait_warp(&empty[s], ((it / C::NS) & 1) ^ 1, abort_flag, lane, 0)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t xs = sbase + s * C::STAGE, ws = xs + C::X_STAGE, bar = smem_u32(&full[s]);
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&full[s], bytes);
+                        tma_load_3d(ws, &tm_w, b * F8B, tile.m0, tile.expert, bar);
+                    }
+                    __syncwarp();
+                    if constexpr (GATHER) {
+                        if (lane < quads) tma_gather4(xs + lane * 4 * F8B, &tm_x, b * F8B, r[0], r[1], r[2], r[3], bar);
+                    } else {
+                        if (lane < boxes) tma_load_2d(xs + lane * G_XBOX * F8B, &tm_x, b * F8B, tile.row0 + lane * G_XBOX, bar);
+                    }
+                }
+            }
+            if (*abort_flag)  // let the copies in flight land before the CTA exits
+                for (int i = max(0, it - C::NS); i < it; i++) mbar_wait_bounded(&full[i % C::NS], (i / C::NS) & 1);
+        } else if (warp == 1) {
+            // ---- MMA issuer -----------------------------------------------------
+            constexpr uint32_t idesc = f8_idesc(GM, BN);
+            int it = 0;
+            bool ok = true;
+            for (int t = t0; ok; t += t_step) {
+                const GTile tile = g_tile(q, start, t, BN);
+                if (tile.expert < 0) break;
+                if (lane == 0) {
+                    for (int b = b0; b < b1; b++, it++) {
+                        const int s = it % C::NS, u = it % C::NB;
+                        if (!tc_wait(&t_empty[u], ((it / C::NB) & 1) ^ 1, abort_flag) ||
+                            !tc_wait(&full[s], (it / C::NS) & 1, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t xs = sbase + s * C::STAGE, ws = xs + C::X_STAGE, d = tmem + (uint32_t)(u * BN);
+#pragma unroll
+                        for (int k = 0; k < F8B / 32; k++)
+                            mma_f8f6f4(d, sw128_desc(xs + k * 32), sw128_desc(ws + k * 32), idesc, k ? 1u : 0u);
+                        tc_commit(smem_u32(&empty[s]));
+                        tc_commit(smem_u32(&t_full[u]));
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            }
+            if (lane == 0) tc_commit(smem_u32(drained));  // every MMA issued here
+        }
+    } else {
+        // ---- promotion and output -------------------------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G_REGS_EPI));
+        const int ew = warp - 4, part = ew & 3, half = ew >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + (uint32_t)(half * C::COLS);
+        const uint32_t stage = sbase + C::OFF_OUT + ew * 2048;
+        int it = 0;
+        bool ok = true;
+        for (int t = t0; ok; t += t_step) {
+            const GTile tile = g_tile(q, start, t, BN);
+            if (tile.expert < 0) break;
+            const int r_first = part * 32, row = r_first + lane;
+            const bool any = r_first < tile.rows;  // (warp-uniform)
+            int src = -1;
+            if (row < tile.rows) src = p.g.counts ? f8_source(p.g, tile.row0 + row, p.status) : tile.row0 + row;
+            const float *xr = reinterpret_cast<const float *>(p.xs + (uint64_t)max(src, 0) * p.xs_nb1);
+            // a warpgroup's columns lie in one block row of the weights
+            const int mb = min((tile.m0 + half * C::COLS) / F8B, (p.M - 1) / F8B);
+            const float *wr = reinterpret_cast<const float *>(p.ws + (uint64_t)tile.expert * p.ws_nb2 + (uint64_t)mb * p.ws_nb1);
+            uint64_t acc[C::COLS / 2];
+#pragma unroll
+            for (int i = 0; i < C::COLS / 2; i++) acc[i] = 0;
+            float xv = 0.0f, wv = 0.0f;
+            if (any && b0 < b1) {
+                xv = xr[b0];
+                wv = wr[b0];
+            }
+            for (int b = b0; b < b1; b++, it++) {
+                const int u = it % C::NB;
+                if (!tc_wait_warp(&t_full[u], (it / C::NB) & 1, abort_flag, lane, 0)) {
+                    ok = false;
+                    break;
+                }
+                if (any) {
+                    tc_fence_after();
+                    const float sc = xv * wv;
+                    const uint64_t sc2 = f2_pack(sc, sc);
+                    if (b + 1 < b1) {  // the next block's scales arrive behind this block's arithmetic
+                        xv = xr[b + 1];
+                        wv = wr[b + 1];
+                    }
+                    uint32_t v[2][32];
+                    tc_ld32(lanes + (uint32_t)(u * BN), v[0]);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < C::COLS / 32; c++) {
+                        if (c + 1 < C::COLS / 32) tc_ld32(lanes + (uint32_t)(u * BN + (c + 1) * 32), v[(c + 1) & 1]);
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            acc[c * 16 + i] = f2_fma(f2_pack_bits(v[c & 1][2 * i], v[c & 1][2 * i + 1]), sc2, acc[c * 16 + i]);
+                        if (c + 1 < C::COLS / 32) tc_wait_ld();
+                    }
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&t_empty[u]);
+            }
+            float f[C::COLS];
+#pragma unroll
+            for (int i = 0; i < C::COLS / 2; i++) f2_unpack(acc[i], f[2 * i], f[2 * i + 1]);
+            if (src < 0) {
+#pragma unroll
+                for (int i = 0; i < C::COLS; i++) f[i] = 0.0f;
+            }
+            if constexpr (SPLIT) {
+                // the pipeline's stages are free: every copy was consumed and every MMA has been read
+                float *mine = reinterpret_cast<float *>(gbase) + row * (BN + 4) + half * C::COLS;
+                if (row < tile.rows) {
+#pragma unroll
+                    for (int i = 0; i < C::COLS; i += 4)
+                        *reinterpret_cast<float4 *>(mine + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                }
+            } else if (ok && any) {
+                const int m0 = tile.m0 + half * C::COLS;
+                const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | p.y_nb1) & 15) == 0;
+                if (p.out_type == FB_F32)
+                    store_rows<float, C::COLS>(f, stage, tile, r_first, m0, p, lane, wide);
+                else if (p.out_type == FB_F16)
+                    store_rows<__half, C::COLS>(f, stage, tile, r_first, m0, p, lane, wide);
+                else
+                    store_rows<__nv_bfloat16, C::COLS>(f, stage, tile, r_first, m0, p, lane, wide);
+            }
+        }
+    }
+    __syncthreads();
+    if constexpr (SPLIT) {
+        cluster_arrive();
+        cluster_wait();
+        const GTile tile = g_tile(q, start, t0, BN);
+        if (warp >= 4 && tile.expert >= 0 && !*abort_flag) {
+            // rows rank, rank + S, ... : the S partial rows added in rank order
+            const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | p.y_nb1) & 15) == 0;
+            for (int r = rank + (warp - 4) * S; r < tile.rows; r += G_EPI_WARPS * S) {
+                for (int c = lane * 8; c < BN; c += 256) {
+                    float f[8] = {};
+                    for (int i = 0; i < S; i++) {
+                        const uint32_t a = dsmem_map(gbase + (r * (BN + 4) + c) * 4, (uint32_t)i);
+                        const int4 lo = dsmem_ld16(a), hi = dsmem_ld16(a + 16);
+                        const int w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                        for (int j = 0; j < 8; j++) f[j] += __int_as_float(w[j]);
+                    }
+                    const int m = tile.m0 + c;
+                    uint8_t *o = p.y + (uint64_t)(tile.row0 + r) * p.y_nb1;
+                    if (m < p.M) {
+                        if (p.out_type == FB_F32) {
+                            store16<float>(o, m, p.M, pack16<float>(f), wide);
+                            if (m + 4 < p.M) store16<float>(o, m + 4, p.M, pack16<float>(f + 4), wide);
+                        } else if (p.out_type == FB_F16) {
+                            store16<__half>(o, m, p.M, pack16<__half>(f), wide);
+                        } else {
+                            store16<__nv_bfloat16>(o, m, p.M, pack16<__nv_bfloat16>(f), wide);
+                        }
+                    }
+                }
+            }
+        }
+        cluster_arrive();
+        cluster_wait();
+    }
+    if (*abort_flag && tid == 0) report_status(p.status, STATUS_TIMEOUT);
+    if (warp == 2) {
+        mbar_wait_bounded(drained, 0);
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int BN, bool SPLIT, bool GATHER>
+int launch_t(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const GParams &q, int ctas, int cluster, cudaStream_t s) {
+    using C = GCfg<BN>;
+    auto *fn = gemm_f8_kernel<BN, SPLIT, GATHER>;
+    static DeviceFlags done;
+    int rc = raise_smem_limit(reinterpret_cast<const void *>(fn), C::BYTES, done, "mul_mat_f8");
+    if (rc) return rc;
+    // setmaxnreg draws on the registers of the launch: the two shares must fit
+    static const int regs = [] {
+        cudaFuncAttributes a{};
+        return cudaFuncGetAttributes(&a, reinterpret_cast<const void *>(gemm_f8_kernel<BN, SPLIT, GATHER>)) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (regs * G_THREADS < 256 * G_REGS_EPI + 128 * G_REGS_REST)
+        return fb::set_error(FB_ERR_CUDA, "mul_mat_f8: built with %d registers per thread", regs);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(G_THREADS);
+    cfg.dynamicSmemBytes = C::BYTES;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = SPLIT ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tm_w, tm_x, q);
+    if (e != cudaSuccess) return fb::set_error(FB_ERR_CUDA, "mul_mat_f8 launch: %s", cudaGetErrorString(e));
+    return FB_OK;
+}
+
+template <int BN, bool SPLIT>
+int launch_g(bool gather, const CUtensorMap &tm_w, const CUtensorMap &tm_x, const GParams &q, int ctas, int cluster,
+             cudaStream_t s) {
+    return gather ? launch_t<BN, SPLIT, true>(tm_w, tm_x, q, ctas, cluster, s)
+                  : launch_t<BN, SPLIT, false>(tm_w, tm_x, q, ctas, cluster, s);
+}
+
+}  // namespace
+
+bool gemm_f8_supported(const F8Gemm &p) {
+    auto ok = [](const void *a, uint64_t nb) { return ((reinterpret_cast<uintptr_t>(a) | nb) & 15) == 0 && nb < (1ull << 40); };
+    if (!ok(p.w, p.w_nb1) || !ok(p.x, p.x_nb1)) return false;
+    // planes of experts, one behind the other
+    return p.g.n_experts <= 1 || (p.w_nb2 % 16 == 0 && p.w_nb2 < (1ull << 40) && p.w_nb2 >= (uint64_t)p.M * p.w_nb1);
+}
+
+int launch_gemm_f8(const F8Gemm &p, cudaStream_t s) {
+    const bool grouped = p.g.counts != nullptr, gather = grouped && p.g.rows;
+    const int sms = sm_count();
+    const int64_t n_exp = grouped ? p.g.n_experts : 1;
+    const int64_t m128 = (p.M + 127) / 128, m256 = (p.M + 255) / 256;
+    // row tiles: exact, or the most that the groups can need
+    const int64_t nt = grouped ? std::min<int64_t>(p.N, p.N / GM + std::min<int64_t>(n_exp, p.N)) : (p.N + GM - 1) / GM;
+    GParams q{};
+    q.p = p;
+    q.kb = (p.K + F8B - 1) / F8B;
+    q.tiles_n = (int)nt;
+    q.band = 16;
+    if (nt * m128 > INT32_MAX / 2) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: too many tiles");
+    const int bn = nt * m256 >= sms ? 256 : 128;
+    const int64_t tiles = nt * (bn == 256 ? m256 : m128);
+    q.tiles_m = (int)(bn == 256 ? m256 : m128);
+    int split = 1;
+    if (bn == 128)
+        while (split < 8 && tiles * split * 2 <= sms && q.kb / (split * 2) >= 2) split *= 2;
+    CUtensorMap tm_w, tm_x;
+    int rc = encode_tensor_map_3d_sw128(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, (uint64_t)p.K, (uint64_t)p.M,
+                                        (uint64_t)n_exp, p.w_nb1, n_exp > 1 ? p.w_nb2 : p.w_nb1 * (uint64_t)p.M, F8B,
+                                        (uint32_t)bn);
+    if (rc) return rc;
+    rc = encode_tensor_map_2d_sw128(&tm_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.x, (uint64_t)p.K,
+                                    (uint64_t)(grouped ? p.g.n_x : p.N), p.x_nb1, F8B, gather ? 1 : G_XBOX);
+    if (rc) return rc;
+    if (split > 1) return launch_g<128, true>(gather, tm_w, tm_x, q, (int)tiles * split, split, s);
+    const int ctas = (int)std::min<int64_t>(tiles, sms);
+    if (bn == 256) return launch_g<256, false>(gather, tm_w, tm_x, q, ctas, 1, s);
+    return launch_g<128, false>(gather, tm_w, tm_x, q, ctas, 1, s);
+}
+
+}  // namespace fbk

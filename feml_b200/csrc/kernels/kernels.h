@@ -264,6 +264,9 @@ struct F8Gemm {
 };
 // gemm_f8_any.cu: any alignment.
 int launch_gemm_f8_any(const F8Gemm &p, cudaStream_t s);
+// gemm_f8.cu: tcgen05 tiles fed by TMA (16-byte aligned rows).
+bool gemm_f8_supported(const F8Gemm &p);
+int launch_gemm_f8(const F8Gemm &p, cudaStream_t s);
 
 int sm_count();
 

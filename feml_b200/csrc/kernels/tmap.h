@@ -16,6 +16,11 @@ int encode_tensor_map_2d(CUtensorMap *map, CUtensorMapDataType dt, const void *b
 int encode_tensor_map_2d_sw128(CUtensorMap *map, CUtensorMapDataType dt, const void *base, uint64_t dim0,
                                uint64_t dim1, uint64_t stride1, uint32_t box0, uint32_t box1);
 
+// Rank 3: dim2 planes, stride2 bytes apart (a multiple of 16); boxes of one plane.
+int encode_tensor_map_3d_sw128(CUtensorMap *map, CUtensorMapDataType dt, const void *base, uint64_t dim0,
+                               uint64_t dim1, uint64_t dim2, uint64_t stride1, uint64_t stride2, uint32_t box0,
+                               uint32_t box1);
+
 #ifdef __CUDACC__
 // One 2D box into shared memory, completing on `bar` (no multicast). The
 // innermost coordinate times the element size must be a multiple of 16 bytes.
