@@ -11,9 +11,17 @@
 // Roles of a CTA of 384 threads, one per SM, persistent over tiles of 128
 // rows x BN weight rows:
 //   warp 0      TMA producer: 128 x 128 bytes of x and BN x 128 bytes of w per
-//               stage (128-byte swizzle); gathered rows with tile::gather4
+//               stage (128-byte swizzle)
 //   warp 1      issues the MMAs of a block into one of 512 / BN TMEM buffers
 //   warp 2      allocates TMEM
+//   warp 2      also copies the block scales of the tile's rows and weights into
+//               shared memory, transposed, eight blocks at a time (read by the
+//               epilogue threads straight from global memory, a row each, they
+//               cost more than the MMAs: 32 cache lines per load)
+//   warp 3      gate: waits for the sums of a block and lets the epilogue warps
+//               through a named barrier (a dozen warps polling shared-memory
+//               barriers slow down every barrier operation: a poll of a
+//               completed barrier went from 50 to 340 cycles)
 //   warps 4-11  promote: two warpgroups, BN / 2 columns each; at a tile's end
 //               they round, transpose through shared memory and store rows
 // A 128 x 256 tile needs 512 cycles of MMA per block; reading its 32768
@@ -42,11 +50,19 @@ namespace fbk {
 namespace {
 
 constexpr int GM = 128;           // rows per tile
-constexpr int G_THREADS = 384;
-constexpr int G_EPI_WARPS = 8;
+#ifndef G_EPI_WARPS_
+#define G_EPI_WARPS_ 8
+#endif
+constexpr int G_EPI_WARPS = G_EPI_WARPS_;
+constexpr int G_EPI_GROUPS = G_EPI_WARPS / 4;
+constexpr int G_THREADS = 128 + 32 * G_EPI_WARPS;
 constexpr int G_XBOX = 32;        // rows per TMA box of x: only boxes with live rows are fetched
 constexpr int G_MAX_E = 1024;
-constexpr int G_REGS_EPI = 216, G_REGS_REST = 40;
+constexpr int G_REGS_EPI = G_EPI_WARPS == 8 ? 208 : 104, G_REGS_REST = G_EPI_WARPS == 8 ? 88 : 64;
+constexpr int G_SCB = 8;          // blocks per chunk of scales
+constexpr int G_SCR = 3;          // chunks in flight
+constexpr int G_SCP = GM + 4;     // floats between two blocks of a chunk (the copy to it has no bank conflicts)
+constexpr int G_STG = 32;         // bytes of a row that an epilogue warp stages at a time
 
 template <int BN>
 struct GCfg {
@@ -55,11 +71,13 @@ struct GCfg {
     static constexpr int STAGE = X_STAGE + W_STAGE;
     static constexpr int NS = BN == 256 ? 4 : 6;  // stages
     static constexpr int NB = 512 / BN;           // TMEM buffers
-    static constexpr int COLS = BN / 2;           // columns per epilogue warpgroup
-    static constexpr int OFF_OUT = NS * STAGE;    // 2 KB per epilogue warp
-    static constexpr int OFF_GRP = OFF_OUT + G_EPI_WARPS * 2048;
-    static constexpr int OFF_BAR = OFF_GRP + (G_MAX_E + 1) * 4 + 12;
-    static constexpr int BYTES = OFF_BAR + (2 * NS + 2 * NB + 1) * 8 + 16 + 1024;
+    static constexpr int COLS = BN / G_EPI_GROUPS;  // columns per epilogue warpgroup
+    static constexpr int OFF_OUT = NS * STAGE;    // 32 rows of G_STG bytes per epilogue warp
+    static constexpr int OFF_GRP = OFF_OUT + G_EPI_WARPS * 32 * G_STG;
+    static constexpr int OFF_SX = OFF_GRP + (G_MAX_E + 1) * 4 + 12;
+    static constexpr int OFF_SW = OFF_SX + G_SCR * G_SCB * G_SCP * 4;
+    static constexpr int OFF_BAR = OFF_SW + G_SCR * G_SCB * 2 * 4;
+    static constexpr int BYTES = OFF_BAR + (2 * NS + 2 * NB + 2 * G_SCR + 1) * 8 + 16 + 1024;
     static_assert(OFF_BAR % 8 == 0 && BYTES <= 232448, "shared memory");
     static_assert(GM * (BN + 4) * 4 <= NS * STAGE, "partial tile of a split");
 };
@@ -87,6 +105,27 @@ __device__ __forceinline__ void mma_f8f6f4(uint32_t d, uint64_t adesc, uint64_t 
 // Instruction descriptor, kind::f8f6f4: D f32, A and B e4m3, both K-major.
 constexpr uint32_t f8_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 
+// The gate warp and the epilogue warps meet once per block.
+__device__ __forceinline__ void gate_sync() {
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * (G_EPI_WARPS + 1)) : "memory");
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// Four bytes into shared memory (zero where n = 0), and the arrival of this
+// thread's copies so far on a barrier.
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // Four rows (any four) of one 128-byte column box.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, int c0, int r0, int r1, int r2, int r3,
                                             uint32_t bar) {
@@ -95,6 +134,18 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map
         "%5, %6}], [%7];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
         : "memory");
+}
+
+// Bounded wait of a whole warp.
+__device__ __forceinline__ bool tc_wait_all(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    bool ok = false;
+    for (uint32_t i = 0; i < kWaitLimit; i++) {
+        ok = mbar_try_wait(bar, parity);
+        if (ok || ((i & 63u) == 63u && *abort_flag)) break;
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) *abort_flag = 1;
+    return ok;
 }
 
 // Tile `t` (expert < 0 past the last). Ungrouped: bands of row tiles, all
@@ -153,30 +204,30 @@ __device__ __forceinline__ void store16(uint8_t *row, int m, int M, uint4 v, boo
     }
 }
 
-// One warp's 32 rows x COLS columns of finished sums (a row per lane): 64
-// bytes of each row at a time through 2 KB of shared memory, so that the
+// One warp's 32 rows x COLS columns of finished sums (a row per lane): 32
+// bytes of each row at a time through 1 KB of shared memory, so that the
 // global stores cover whole sectors. 16-byte unit u of row r lies at
-// u ^ ((r >> 1) & 3): neither side has bank conflicts.
+// u ^ ((r >> 2) & 1): neither side has bank conflicts.
 template <typename T, int COLS>
 __device__ __forceinline__ void store_rows(const float (&acc)[COLS], uint32_t stage, const GTile &t, int r_first, int m0,
                                            const F8Gemm &p, int lane, bool wide) {
     constexpr int N = Vec<T>::N;
 #pragma unroll
-    for (int c = 0; c < COLS; c += 4 * N) {
+    for (int c = 0; c < COLS; c += 2 * N) {
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < 2; u++) {
             const uint4 v = pack16<T>(&acc[c + u * N]);
-            const uint32_t a = stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4);
+            const uint32_t a = stage + lane * G_STG + ((u ^ ((lane >> 2) & 1)) << 4);
             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
         }
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = i * 8 + (lane >> 2), u = lane & 3;
+        for (int i = 0; i < 2; i++) {
+            const int r = i * 16 + (lane >> 1), u = lane & 1;
             uint4 v;
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                         : "r"(stage + r * 64 + ((u ^ ((r >> 1) & 3)) << 4))
+                         : "r"(stage + r * G_STG + ((u ^ ((r >> 2) & 1)) << 4))
                          : "memory");
             const int m = m0 + c + u * N;
             if (r_first + r < t.rows && m < p.M)
@@ -199,7 +250,11 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     uint64_t *empty = full + C::NS;
     uint64_t *t_full = empty + C::NS;
     uint64_t *t_empty = t_full + C::NB;
-    uint64_t *drained = t_empty + C::NB;
+    uint64_t *s_full = t_empty + C::NB;
+    uint64_t *s_empty = s_full + G_SCR;
+    uint64_t *drained = s_empty + G_SCR;
+    float *sx = reinterpret_cast<float *>(gbase + C::OFF_SX);
+    float *sw = reinterpret_cast<float *>(gbase + C::OFF_SW);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -213,6 +268,10 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         for (int i = 0; i < C::NB; i++) {
             mbar_init(&t_full[i], 1);
             mbar_init(&t_empty[i], G_EPI_WARPS);
+        }
+        for (int i = 0; i < G_SCR; i++) {
+            mbar_init(&s_full[i], 32);
+            mbar_init(&s_empty[i], G_EPI_WARPS);
         }
         mbar_init(drained, 1);
         *abort_flag = 0;
@@ -263,11 +322,11 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                     for (int j = 0; j < 4; j++)
                         if (lane * 4 + j < tile.rows) r[j] = max(0, f8_source(p.g, tile.row0 + lane * 4 + j, nullptr));
                 }
-                const int boxes = (tile.rows + G_XBOX - 1) / G_XBOX, quads = (tile.rows + 3) / 4;
-                const uint32_t bytes = C::W_STAGE + (GATHER ? quads * 4 * F8B : boxes * G_XBOX * F8B);
+                const int boxes = (tile.rows + (GATHER ? 3 : G_XBOX - 1)) / (GATHER ? 4 : G_XBOX);
+                const uint32_t bytes = C::W_STAGE + boxes * (GATHER ? 4 : G_XBOX) * F8B;
                 for (int b = b0; b < b1; b++, it++) {
                     const int s = it % C::NS;
-                    if (!tc_wait_warp(&empty[s], ((it / C::NS) & 1) ^ 1, abort_flag, lane, 0)) {
+                    if (!tc_wait_warp(&empty[s], ((it / C::NS) & 1) ^ 1, abort_flag, lane, 20)) {
                         ok = false;
                         break;
                     }
@@ -277,101 +336,146 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                         tma_load_3d(ws, &tm_w, b * F8B, tile.m0, tile.expert, bar);
                     }
                     __syncwarp();
-                    if constexpr (GATHER) {
-                        if (lane < quads) tma_gather4(xs + lane * 4 * F8B, &tm_x, b * F8B, r[0], r[1], r[2], r[3], bar);
-                    } else {
-                        if (lane < boxes) tma_load_2d(xs + lane * G_XBOX * F8B, &tm_x, b * F8B, tile.row0 + lane * G_XBOX, bar);
-                    }
+                    if (GATHER) {
+                        if (lane < boxes) tma_gather4(xs + lane * 4 * F8B, &tm_x, b * F8B, r[0], r[1], r[2], r[3], bar);
+                    } else if (lane < boxes) tma_load_2d(xs + lane * G_XBOX * F8B, &tm_x, b * F8B, tile.row0 + lane * G_XBOX, bar);
                 }
             }
             if (*abort_flag)  // let the copies in flight land before the CTA exits
                 for (int i = max(0, it - C::NS); i < it; i++) mbar_wait_bounded(&full[i % C::NS], (i / C::NS) & 1);
         } else if (warp == 1) {
             // ---- MMA issuer -----------------------------------------------------
+            // (the whole warp walks the loop and one elected lane issues: with
+            // warp-uniform operands an MMA issues in a few cycles, from a
+            // divergent branch in about 50)
             constexpr uint32_t idesc = f8_idesc(GM, BN);
+            const uint64_t desc0 = sw128_desc(sbase);
             int it = 0;
+            bool ok = true;
+            for (int t = t0; ok; t += t_step) {
+                if (g_tile(q, start, t, BN).expert < 0) break;
+                for (int b = b0; b < b1; b++, it++) {
+                    const int s = it % C::NS, u = it % C::NB;
+                    if (!tc_wait_all(&full[s], (it / C::NS) & 1, abort_flag) ||
+                        !tc_wait_all(&t_empty[u], ((it / C::NB) & 1) ^ 1, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t xd = desc0 + (uint64_t)(s * (C::STAGE / 16)), wd = xd + C::X_STAGE / 16;
+                    const uint32_t d = tmem + (uint32_t)(u * BN);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < F8B / 32; k++) mma_f8f6f4(d, xd + k * 2, wd + k * 2, idesc, k ? 1u : 0u);
+                        tc_commit(smem_u32(&t_full[u]));
+                        tc_commit(smem_u32(&empty[s]));
+                    }
+                    __syncwarp();
+                }
+            }
+            if (elect_one()) tc_commit(smem_u32(drained));  // every MMA issued here
+        } else if (warp == 2) {
+            // ---- scales: G_SCB blocks of 128 rows at a time, eight lanes per row -------------
+            const int j = lane & 7;
+            int ch = 0;
             bool ok = true;
             for (int t = t0; ok; t += t_step) {
                 const GTile tile = g_tile(q, start, t, BN);
                 if (tile.expert < 0) break;
-                if (lane == 0) {
-                    for (int b = b0; b < b1; b++, it++) {
-                        const int s = it % C::NS, u = it % C::NB;
-                        if (!tc_wait(&t_empty[u], ((it / C::NB) & 1) ^ 1, abort_flag) ||
-                            !tc_wait(&full[s], (it / C::NS) & 1, abort_flag)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t xs = sbase + s * C::STAGE, ws = xs + C::X_STAGE, d = tmem + (uint32_t)(u * BN);
+                int src[4];  // scale rows of tile rows lane, 32 + lane, ...
 #pragma unroll
-                        for (int k = 0; k < F8B / 32; k++)
-                            mma_f8f6f4(d, sw128_desc(xs + k * 32), sw128_desc(ws + k * 32), idesc, k ? 1u : 0u);
-                        tc_commit(smem_u32(&empty[s]));
-                        tc_commit(smem_u32(&t_full[u]));
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const int r = i * 32 + lane;
+                    src[i] = -1;
+                    if (r < tile.rows) src[i] = p.g.counts ? f8_source(p.g, tile.row0 + r, nullptr) : tile.row0 + r;
                 }
-                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                const int mb = tile.m0 / F8B + (lane >> 3), mbs = (p.M + F8B - 1) / F8B;
+                const uint8_t *wr = p.ws + (uint64_t)tile.expert * p.ws_nb2 + (uint64_t)min(mb, mbs - 1) * p.ws_nb1;
+                for (int b = b0; b < b1; b += G_SCB, ch++) {
+                    const int c = ch % G_SCR;
+                    if (!tc_wait_warp(&s_empty[c], ((ch / G_SCR) & 1) ^ 1, abort_flag, lane, 100)) {
+                        ok = false;
+                        break;
+                    }
+                    const bool in = b + j < b1;
+                    if (lane < 16 && in) cp_async4(smem_u32(&sw[(c * G_SCB + j) * 2 + (lane >> 3)]), wr + (b + j) * 4, 4);
+                    const uint32_t dst = smem_u32(&sx[(c * G_SCB + j) * G_SCP + (lane >> 3)]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int r = __shfl_sync(0xffffffffu, src[i], e * 4 + (lane >> 3));
+                            const bool get = r >= 0 && in;
+                            cp_async4(dst + (i * 32 + e * 4) * 4, p.xs + (get ? (uint64_t)r * p.xs_nb1 + (b + j) * 4 : 0), get ? 4 : 0);
+                        }
+                    }
+                    cp_async_arrive(&s_full[c]);
+                }
             }
-            if (lane == 0) tc_commit(smem_u32(drained));  // every MMA issued here
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+            // ---- gate: waits for a block's sums (and scales) on the epilogue's behalf --------------
+            // (after an abort it lets every remaining step through without waiting)
+            int it = 0, ch = 0;
+            bool ok = true;
+            for (int t = t0;; t += t_step) {
+                if (g_tile(q, start, t, BN).expert < 0) break;
+                for (int b = b0; b < b1; b++, it++) {
+                    const int u = it % C::NB;
+                    if ((b - b0) % G_SCB == 0) {
+                        ok = ok && tc_wait_all(&s_full[ch % G_SCR], (ch / G_SCR) & 1, abort_flag);
+                        ch++;
+                    }
+                    ok = ok && tc_wait_all(&t_full[u], (it / C::NB) & 1, abort_flag);
+                    gate_sync();
+                }
+            }
         }
     } else {
         // ---- promotion and output -------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G_REGS_EPI));
-        const int ew = warp - 4, part = ew & 3, half = ew >> 2;
-        const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + (uint32_t)(half * C::COLS);
-        const uint32_t stage = sbase + C::OFF_OUT + ew * 2048;
-        int it = 0;
-        bool ok = true;
-        for (int t = t0; ok; t += t_step) {
+        const int ew = warp - 4, part = ew & 3, grp = ew >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + (uint32_t)(grp * C::COLS);
+        const uint32_t stage = sbase + C::OFF_OUT + ew * 32 * G_STG;
+        int it = 0, ch = 0;
+        for (int t = t0;; t += t_step) {
             const GTile tile = g_tile(q, start, t, BN);
             if (tile.expert < 0) break;
             const int r_first = part * 32, row = r_first + lane;
             const bool any = r_first < tile.rows;  // (warp-uniform)
-            int src = -1;
-            if (row < tile.rows) src = p.g.counts ? f8_source(p.g, tile.row0 + row, p.status) : tile.row0 + row;
-            const float *xr = reinterpret_cast<const float *>(p.xs + (uint64_t)max(src, 0) * p.xs_nb1);
-            // a warpgroup's columns lie in one block row of the weights
-            const int mb = min((tile.m0 + half * C::COLS) / F8B, (p.M - 1) / F8B);
-            const float *wr = reinterpret_cast<const float *>(p.ws + (uint64_t)tile.expert * p.ws_nb2 + (uint64_t)mb * p.ws_nb1);
             uint64_t acc[C::COLS / 2];
 #pragma unroll
             for (int i = 0; i < C::COLS / 2; i++) acc[i] = 0;
-            float xv = 0.0f, wv = 0.0f;
-            if (any && b0 < b1) {
-                xv = xr[b0];
-                wv = wr[b0];
-            }
             for (int b = b0; b < b1; b++, it++) {
-                const int u = it % C::NB;
-                if (!tc_wait_warp(&t_full[u], (it / C::NB) & 1, abort_flag, lane, 0)) {
-                    ok = false;
-                    break;
-                }
+                const int u = it % C::NB, j = (b - b0) % G_SCB, c = ch % G_SCR;
+                gate_sync();
+                // a warpgroup's columns lie in one block row of the weights
+                const float sc = sx[(c * G_SCB + j) * G_SCP + row] * sw[(c * G_SCB + j) * 2 + grp * C::COLS / F8B];
                 if (any) {
                     tc_fence_after();
-                    const float sc = xv * wv;
                     const uint64_t sc2 = f2_pack(sc, sc);
-                    if (b + 1 < b1) {  // the next block's scales arrive behind this block's arithmetic
-                        xv = xr[b + 1];
-                        wv = wr[b + 1];
-                    }
-                    uint32_t v[2][32];
-                    tc_ld32(lanes + (uint32_t)(u * BN), v[0]);
+                    uint32_t v[2][16];
+                    tc_ld16(lanes + (uint32_t)(u * BN), v[0]);
                     tc_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < C::COLS / 32; c++) {
-                        if (c + 1 < C::COLS / 32) tc_ld32(lanes + (uint32_t)(u * BN + (c + 1) * 32), v[(c + 1) & 1]);
+                    for (int h = 0; h < C::COLS / 16; h++) {
+                        if (h + 1 < C::COLS / 16) tc_ld16(lanes + (uint32_t)(u * BN + (h + 1) * 16), v[(h + 1) & 1]);
 #pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            acc[c * 16 + i] = f2_fma(f2_pack_bits(v[c & 1][2 * i], v[c & 1][2 * i + 1]), sc2, acc[c * 16 + i]);
-                        if (c + 1 < C::COLS / 32) tc_wait_ld();
+                        for (int i = 0; i < 8; i++)
+                            acc[h * 8 + i] = f2_fma(f2_pack_bits(v[h & 1][2 * i], v[h & 1][2 * i + 1]), sc2, acc[h * 8 + i]);
+                        if (h + 1 < C::COLS / 16) tc_wait_ld();
                     }
                     tc_fence_before();
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t_empty[u]);
+                if (j == G_SCB - 1 || b == b1 - 1) {
+                    if (lane == 0) mbar_arrive(&s_empty[c]);
+                    ch++;
+                }
             }
+            int src = -1;
+            if (row < tile.rows) src = p.g.counts ? f8_source(p.g, tile.row0 + row, p.status) : 0;
             float f[C::COLS];
 #pragma unroll
             for (int i = 0; i < C::COLS / 2; i++) f2_unpack(acc[i], f[2 * i], f[2 * i + 1]);
@@ -381,14 +485,14 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             }
             if constexpr (SPLIT) {
                 // the pipeline's stages are free: every copy was consumed and every MMA has been read
-                float *mine = reinterpret_cast<float *>(gbase) + row * (BN + 4) + half * C::COLS;
+                float *mine = reinterpret_cast<float *>(gbase) + row * (BN + 4) + grp * C::COLS;
                 if (row < tile.rows) {
 #pragma unroll
                     for (int i = 0; i < C::COLS; i += 4)
                         *reinterpret_cast<float4 *>(mine + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
                 }
-            } else if (ok && any) {
-                const int m0 = tile.m0 + half * C::COLS;
+            } else if (any && !*abort_flag) {
+                const int m0 = tile.m0 + grp * C::COLS;
                 const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | p.y_nb1) & 15) == 0;
                 if (p.out_type == FB_F32)
                     store_rows<float, C::COLS>(f, stage, tile, r_first, m0, p, lane, wide);
@@ -456,7 +560,7 @@ int launch_t(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const GParams &q,
         cudaFuncAttributes a{};
         return cudaFuncGetAttributes(&a, reinterpret_cast<const void *>(gemm_f8_kernel<BN, SPLIT, GATHER>)) == cudaSuccess ? a.numRegs : 0;
     }();
-    if (regs * G_THREADS < 256 * G_REGS_EPI + 128 * G_REGS_REST)
+    if (regs * G_THREADS < 32 * G_EPI_WARPS * G_REGS_EPI + 128 * G_REGS_REST)
         return fb::set_error(FB_ERR_CUDA, "mul_mat_f8: built with %d registers per thread", regs);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)ctas);
