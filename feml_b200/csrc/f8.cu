@@ -57,9 +57,13 @@ int check_out(const char *op, const fbk::F8Out &o, int64_t rows, int64_t k, int6
 // A row stride that no second row uses must not decide alignment.
 uint64_t stride_of(uint64_t nb1, int64_t rows, int64_t bytes) { return rows > 1 ? nb1 : (uint64_t)(bytes + 15) / 16 * 16; }
 
-int run_product(const fbk::F8Gemm &p, cudaStream_t s) {
-    if (fbk::gemm_f8_supported(p)) return fbk::launch_gemm_f8(p, s);
-    return fbk::launch_gemm_f8_any(p, s);
+int run_product(fbk::F8Gemm &p, void *ws, uint64_t ws_bytes, cudaStream_t s) {
+    if (!fbk::gemm_f8_supported(p)) return fbk::launch_gemm_f8_any(p, s);
+    if (!p.g.counts && p.N <= fbk::gemv_f8_max_rows()) return fbk::launch_gemv_f8(p, s);
+    if (p.g.rows && fbk::gather_f8_pays(p.g.n_rows, p.g.n_experts) && ws && !off(ws, 0, 16) &&
+        ws_bytes >= fbk::gather_f8_bytes(p.K, p.g.n_rows))
+        FB_TRY(fbk::launch_gather_f8(p, ws, s));
+    return fbk::launch_gemm_f8(p, s);
 }
 
 // K = 0: every sum is empty.
@@ -160,7 +164,16 @@ int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, ui
     p.K = (int)K;
     p.M = (int)M;
     p.N = (int)N;
-    return run_product(p, s);
+    return run_product(p, nullptr, 0, s);
+}
+
+int feml_b200_mul_mat_f8_grouped_workspace(int64_t K, int64_t n_rows, int64_t n_experts, uint64_t *bytes) {
+    const char *op = "mul_mat_f8_grouped_workspace";
+    if (!bytes) return set_error(FB_ERR_INVALID, "%s: null out", op);
+    *bytes = 0;
+    FB_TRY(check_dims(op, K, n_rows, n_experts));
+    if (fbk::gather_f8_pays(n_rows, n_experts)) *bytes = fbk::gather_f8_bytes(K, n_rows);
+    return FB_OK;
 }
 
 int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, const float *w_scale,
@@ -168,7 +181,8 @@ int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, 
                                  uint64_t x_nb1, int64_t n_x, const float *x_scale, uint64_t x_scale_nb1,
                                  const int32_t *counts, const int32_t *offsets, const int32_t *rows,
                                  int64_t n_selected, int32_t dst_type, void *dst, uint64_t dst_nb1, int64_t K,
-                                 int64_t M, int64_t n_rows, int32_t *status, void *stream) {
+                                 int64_t M, int64_t n_rows, void *workspace, uint64_t workspace_bytes, int32_t *status,
+                                 void *stream) {
     const char *op = "mul_mat_f8_grouped";
     FB_TRY(check_type(op, dst_type));
     FB_TRY(check_dims(op, K, M, n_rows));
@@ -219,7 +233,7 @@ int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, 
     p.g.n_selected = (int)n_selected;
     p.g.n_x = (int)n_x;
     p.status = status;
-    return run_product(p, static_cast<cudaStream_t>(stream));
+    return run_product(p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

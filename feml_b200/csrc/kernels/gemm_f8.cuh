@@ -44,6 +44,19 @@ __device__ __forceinline__ int f8_source(const F8Groups &g, int r, int32_t *stat
     return t;
 }
 
+// The row of the caller's x behind grouped row r, as f8_source, whether the
+// rows are gathered by the product itself or were beforehand.
+__device__ __forceinline__ int f8_origin(const F8Groups &g, int r, int32_t *status) {
+    if (!g.gathered) return f8_source(g, r, status);
+    const int i = g.gathered[r];
+    const int t = i < 0 ? -1 : i / g.n_selected;
+    if (t < 0 || t >= g.n_origin) {
+        report_status(status, STATUS_BAD_ID);
+        return -1;
+    }
+    return t;
+}
+
 // The group and row tile (of `bm` rows) behind index `tile` when every group
 // is cut into tiles of its own; expert < 0 past the last one. Called by a
 // whole warp.

@@ -249,6 +249,10 @@ int launch_rms_norm_f8(int32_t type, const void *x, uint64_t x_nb1, const void *
 struct F8Groups {
     const int32_t *counts, *offsets, *rows;
     int n_experts, n_rows, n_selected, n_x;
+    // Row table whose rows were gathered beforehand (rows == null then; row r
+    // of x is row r of dst), for its checks: entries / n_selected < n_origin.
+    const int32_t *gathered;
+    int n_origin;
 };
 // Operands of an e4m3 product: N output rows (grouped: the rows of the
 // output buffer), weight rows at w + e*w_nb2 + m*w_nb1.
@@ -264,9 +268,18 @@ struct F8Gemm {
 };
 // gemm_f8_any.cu: any alignment.
 int launch_gemm_f8_any(const F8Gemm &p, cudaStream_t s);
+// gemv_f8.cu: up to gemv_f8_max_rows() rows of x, ungrouped (16-byte aligned rows).
+int gemv_f8_max_rows();
+int launch_gemv_f8(const F8Gemm &p, cudaStream_t s);
 // gemm_f8.cu: tcgen05 tiles fed by TMA (16-byte aligned rows).
 bool gemm_f8_supported(const F8Gemm &p);
 int launch_gemm_f8(const F8Gemm &p, cudaStream_t s);
+// Rows of x and their scales in the order of a grouped product's row table,
+// written to `ws` (gather_f8_bytes; 16-byte aligned); on return `p` reads
+// them there. Worth a pass of its own from gather_f8_pays on.
+uint64_t gather_f8_bytes(int64_t K, int64_t n_rows);
+bool gather_f8_pays(int64_t n_rows, int64_t n_experts);
+int launch_gather_f8(F8Gemm &p, void *ws, cudaStream_t s);
 
 int sm_count();
 

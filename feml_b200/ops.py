@@ -211,22 +211,35 @@ def block_dots(wtype, w, xq, K):
 # (activations) or per 128 x 128 block (weights); a value is q * scale.
 # ---------------------------------------------------------------------------
 _F8 = torch.float8_e4m3fn
+_F32 = torch.float32
 _F8_TYPES = {torch.float32: 5, torch.float16: 4, torch.bfloat16: 30}
 
+# A decode step is a handful of calls of a few microseconds each, so the
+# checks below read each attribute once and the stream comes as a handle
+# without a Stream object around it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-def _f8_check(op, name, t, dtype, shape, device, like=None):
-    """The tensor of an operand: on `device`, of `dtype` (one of a set or
-    exact), of `shape`, its last dimension contiguous."""
+
+def _f8_refuse(op, name, t, dtype, shape, device):
+    """The reason why `t` is not the operand that a call needs."""
     if not isinstance(t, torch.Tensor):
         raise FemlError("msg", f"{op}: {name} is not a tensor")
-    if t.device != device:
-        raise FemlError("msg", f"{op}: {name} is on {t.device}, not on {device}")
+    if t.get_device() != device:
+        raise FemlError("msg", f"{op}: {name} is on {t.device}, not on cuda:{device}")
     if t.dtype != dtype:
         raise FemlError("unsupported", f"{op}: {name} is {t.dtype}, not {dtype}")
     if tuple(t.shape) != shape:
         raise FemlError("shape", f"{op}: {name} is {list(t.shape)}, not {list(shape)}")
-    if shape[-1] > 1 and t.stride(-1) != 1:
-        raise FemlError("shape", f"{op}: the rows of {name} are not contiguous")
+    raise FemlError("shape", f"{op}: the rows of {name} are not contiguous")
+
+
+def _f8_check(op, name, t, dtype, shape, device):
+    """The tensor of an operand: on CUDA device `device`, of `dtype` and
+    `shape`, its last dimension contiguous."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device
+            and (t.stride(-1) == 1 or shape[-1] <= 1)):
+        _f8_refuse(op, name, t, dtype, shape, device)
 
 
 def _f8_input(op, name, x):
@@ -238,7 +251,7 @@ def _f8_input(op, name, x):
     tid = _F8_TYPES.get(x.dtype)
     if tid is None:
         raise FemlError("unsupported", f"{op}: {name} is {x.dtype} (float32, float16 and bfloat16)")
-    if x.shape[1] > 1 and x.stride(1) != 1:
+    if x.stride(1) != 1 and x.shape[1] > 1:
         raise FemlError("shape", f"{op}: the rows of {name} are not contiguous")
     return tid
 
@@ -247,24 +260,25 @@ def _f8_out(op, out, scale, rows, k, block_rows, device):
     """The two outputs of a quantizing call, given or new."""
     srows, kb = -(-rows // block_rows), -(-k // 128)
     if out is None:
-        out = torch.empty((rows, k), dtype=_F8, device=device)
+        out = torch.empty((rows, k), dtype=_F8, device=f"cuda:{device}")
     else:
         _f8_check(op, "out", out, _F8, (rows, k), device)
     if scale is None:
-        scale = torch.empty((srows, kb), dtype=torch.float32, device=device)
+        scale = torch.empty((srows, kb), dtype=_F32, device=f"cuda:{device}")
     else:
-        _f8_check(op, "scale", scale, torch.float32, (srows, kb), device)
+        _f8_check(op, "scale", scale, _F32, (srows, kb), device)
     return out, scale
 
 
 def _f8_call(device, fn, *args):
     """fn(*args, stream) on `device`'s current stream, with `device` current."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        _check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+    if device == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device))
     else:
-        with torch.cuda.device(index):
-            _check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc:
+        _check(rc)
 
 
 def quantize_f8(x, block_rows=1, out=None, scale=None):
@@ -276,8 +290,8 @@ def quantize_f8(x, block_rows=1, out=None, scale=None):
     if block_rows not in (1, 128):
         raise FemlError("unsupported", f"{op}: blocks of {block_rows} rows (1 or 128)")
     rows, k = x.shape
-    out, scale = _f8_out(op, out, scale, rows, k, block_rows, x.device)
-    _f8_call(x.device, _L.lib().feml_b200_quantize_f8, tid, x.data_ptr(), x.stride(0) * x.element_size(), rows, k,
+    out, scale = _f8_out(op, out, scale, rows, k, block_rows, x.get_device())
+    _f8_call(x.get_device(), _L.lib().feml_b200_quantize_f8, tid, x.data_ptr(), x.stride(0) * x.element_size(), rows, k,
              block_rows, out.data_ptr(), out.stride(0), scale.data_ptr(), scale.stride(0) * 4)
     return out, scale
 
@@ -290,7 +304,7 @@ def rms_norm_f8(x, weight, eps, residual=None, residual_out=None, out=None, scal
     op = "rms_norm_f8"
     tid = _f8_input(op, "x", x)
     rows, k = x.shape
-    dev, es = x.device, x.element_size()
+    dev, es = x.get_device(), x.element_size()
     if isinstance(weight, torch.Tensor) and weight.dtype == torch.float32:
         wid = 5
         _f8_check(op, "weight", weight, torch.float32, (k,), dev)
@@ -301,7 +315,7 @@ def rms_norm_f8(x, weight, eps, residual=None, residual_out=None, out=None, scal
     if residual is not None:
         _f8_check(op, "residual", residual, x.dtype, (rows, k), dev)
         if residual_out is None:
-            residual_out = torch.empty((rows, k), dtype=x.dtype, device=dev)
+            residual_out = torch.empty((rows, k), dtype=x.dtype, device=x.device)
         else:
             _f8_check(op, "residual_out", residual_out, x.dtype, (rows, k), dev)
         r_ptr, r_nb1 = residual.data_ptr(), residual.stride(0) * es
@@ -320,10 +334,11 @@ def silu_mul_f8(gate, up, out=None, scale=None):
     op = "silu_mul_f8"
     tid = _f8_input(op, "gate", gate)
     rows, k = gate.shape
-    _f8_check(op, "up", up, gate.dtype, (rows, k), gate.device)
-    out, scale = _f8_out(op, out, scale, rows, k, 1, gate.device)
+    dev = gate.get_device()
+    _f8_check(op, "up", up, gate.dtype, (rows, k), dev)
+    out, scale = _f8_out(op, out, scale, rows, k, 1, dev)
     es = gate.element_size()
-    _f8_call(gate.device, _L.lib().feml_b200_silu_mul_f8, tid, gate.data_ptr(), gate.stride(0) * es, up.data_ptr(),
+    _f8_call(dev, _L.lib().feml_b200_silu_mul_f8, tid, gate.data_ptr(), gate.stride(0) * es, up.data_ptr(),
              up.stride(0) * es, rows, k, out.data_ptr(), out.stride(0), scale.data_ptr(), scale.stride(0) * 4)
     return out, scale
 
@@ -331,7 +346,7 @@ def silu_mul_f8(gate, up, out=None, scale=None):
 def _f8_dst(op, out, out_dtype, n, m, device):
     """Output of a product and its type id; f32 unless given."""
     if out is None:
-        out = torch.empty((n, m), dtype=out_dtype or torch.float32, device=device)
+        out = torch.empty((n, m), dtype=out_dtype or _F32, device=f"cuda:{device}")
     else:
         _f8_check(op, "out", out, out_dtype or out.dtype, (n, m), device)
     tid = _F8_TYPES.get(out.dtype)
@@ -349,7 +364,7 @@ def mul_mat_f8(w, w_scale, x, x_scale, out=None, out_dtype=None):
         raise FemlError("msg", f"{op}: w is not a 2-dimensional CUDA tensor")
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise FemlError("msg", f"{op}: x is not a 2-dimensional tensor")
-    dev = w.device
+    dev = w.get_device()
     m, k = w.shape
     n, kb = x.shape[0], -(-k // 128)
     _f8_check(op, "w", w, _F8, (m, k), dev)
@@ -363,21 +378,29 @@ def mul_mat_f8(w, w_scale, x, x_scale, out=None, out_dtype=None):
     return out
 
 
+def mul_mat_f8_grouped_workspace(K, n_rows, n_experts):
+    """Workspace bytes for a product of n_rows rows with a row table."""
+    v = ctypes.c_uint64()
+    _check(_L.lib().feml_b200_mul_mat_f8_grouped_workspace(K, n_rows, n_experts, ctypes.byref(v)))
+    return v.value
+
+
 def mul_mat_f8_grouped(w, w_scale, x, x_scale, counts, offsets, rows=None, n_selected=1, out=None, out_dtype=None,
-                       status=None):
+                       workspace=None, status=None):
     """The product for rows grouped by expert: out[r] = expert e's weights
     times row rows[r] // n_selected of x (row r without `rows`), for r in
     [offsets[e], offsets[e] + counts[e]). w e4m3 [E, M, K], w_scale [E,
     ceil(M / 128), ceil(K / 128)], x e4m3 [n, K]; counts, offsets, rows:
     int32 as moe_route gives them. -> [len(rows) or n, M]; rows of `out` in no
-    group are left as they were (zeros when `out` is not given). `status`:
+    group are left as they were (zeros when `out` is not given). `workspace`:
+    uint8, mul_mat_f8_grouped_workspace bytes (allocated when needed). `status`:
     int32 [1], bit 1 is set where a table points outside its range."""
     op = "mul_mat_f8_grouped"
     if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dim() != 3:
         raise FemlError("msg", f"{op}: w is not a 3-dimensional CUDA tensor")
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise FemlError("msg", f"{op}: x is not a 2-dimensional tensor")
-    dev = w.device
+    dev = w.get_device()
     e, m, k = w.shape
     n, kb = x.shape[0], -(-k // 128)
     _f8_check(op, "w", w, _F8, (e, m, k), dev)
@@ -390,21 +413,28 @@ def mul_mat_f8_grouped(w, w_scale, x, x_scale, counts, offsets, rows=None, n_sel
     if rows is not None:
         n_rows = rows.numel() if isinstance(rows, torch.Tensor) else 0
         _f8_check(op, "rows", rows, torch.int32, (n_rows,), dev)
+        if workspace is None:
+            need = mul_mat_f8_grouped_workspace(k, n_rows, e)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=w.device)
+        else:
+            _f8_check(op, "workspace", workspace, torch.uint8, (workspace.numel(),), dev)
     elif n_selected != 1:
         raise FemlError("msg", f"{op}: n_selected = {n_selected} without rows")
     if status is not None:
         _f8_check(op, "status", status, torch.int32, (1,), dev)
     if out is None:
-        out = torch.zeros((n_rows, m), dtype=out_dtype or torch.float32, device=dev)
+        out = torch.zeros((n_rows, m), dtype=out_dtype or _F32, device=w.device)
     out, tid = _f8_dst(op, out, out_dtype, n_rows, m, dev)
     _f8_call(dev, _L.lib().feml_b200_mul_mat_f8_grouped, w.data_ptr(), w.stride(1), w.stride(0), w_scale.data_ptr(),
              w_scale.stride(1) * 4, w_scale.stride(0) * 4, e, x.data_ptr(), x.stride(0), n, x_scale.data_ptr(),
              x_scale.stride(0) * 4, counts.data_ptr(), offsets.data_ptr(), rows.data_ptr() if rows is not None else 0,
              int(n_selected), tid, out.data_ptr(), out.stride(0) * out.element_size(), k, m, n_rows,
+             workspace.data_ptr() if workspace is not None else 0, workspace.numel() if workspace is not None else 0,
              status.data_ptr() if status is not None else 0)
     return out
 
 
 __all__ = ["quantize", "mul_mat", "mul_mat_launches", "mul_mat_workspace", "mul_mat_noalloc", "mul_mat_noalloc_limit", "mul_mat_id", "mul_mat_id_workspace", "mul_mat_id_shard",
            "local_experts", "mul_mat_peer", "mul_mat_id_peer", "peer_wait", "moe_route",
-           "block_dots", "row_bytes", "quantize_f8", "rms_norm_f8", "silu_mul_f8", "mul_mat_f8", "mul_mat_f8_grouped", "FemlError"]
+           "block_dots", "row_bytes", "quantize_f8", "rms_norm_f8", "silu_mul_f8", "mul_mat_f8", "mul_mat_f8_grouped", "mul_mat_f8_grouped_workspace", "FemlError"]

@@ -549,7 +549,14 @@ int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, 
                                  uint64_t x_nb1, int64_t n_x, const float *x_scale, uint64_t x_scale_nb1,
                                  const int32_t *counts, const int32_t *offsets, const int32_t *rows,
                                  int64_t n_selected, int32_t dst_type, void *dst, uint64_t dst_nb1, int64_t K,
-                                 int64_t M, int64_t n_rows, int32_t *status, void *stream);
+                                 int64_t M, int64_t n_rows, void *workspace, uint64_t workspace_bytes,
+                                 int32_t *status, void *stream);
+/* Workspace bytes with which a product with a row table copies the rows of x
+ * into group order first (0 where it would not). Optional: without a
+ * workspace (NULL, too small, or not 16-byte aligned) the rows are fetched
+ * one by one, with the same results. Calls that can overlap need workspaces
+ * of their own. */
+int feml_b200_mul_mat_f8_grouped_workspace(int64_t K, int64_t n_rows, int64_t n_experts, uint64_t *bytes);
 
 /* ---- weight ingestion: host pointers and GGUF files ----------------------- */
 

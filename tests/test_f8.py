@@ -37,9 +37,9 @@ def mul_mat(w=P, w_nb1=256, ws=P, ws_nb1=8, x=P, x_nb1=256, xs=P, xs_nb1=8, t=F3
 
 
 def grouped(w=P, w_nb1=256, w_nb2=256 * 300, ws=P, ws_nb1=8, ws_nb2=24, E=4, x=P, x_nb1=256, n_x=2, xs=P, xs_nb1=8,
-            counts=P, offsets=P, rows=P, sel=1, t=F32, y=P, y_nb1=1200, K=256, M=300, R=2, status=0):
+            counts=P, offsets=P, rows=P, sel=1, t=F32, y=P, y_nb1=1200, K=256, M=300, R=2, work=0, work_n=0, status=0):
     return call("mul_mat_f8_grouped", w, w_nb1, w_nb2, ws, ws_nb1, ws_nb2, E, x, x_nb1, n_x, xs, xs_nb1, counts, offsets,
-                rows, sel, t, y, y_nb1, K, M, R, status, 0)
+                rows, sel, t, y, y_nb1, K, M, R, work, work_n, status, 0)
 
 
 @pytest.mark.parametrize("fn,bad,code", [

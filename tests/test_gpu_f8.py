@@ -358,6 +358,27 @@ def test_grouped(t, counts, k, m, gather):
     assert int(status) == 0
 
 
+@pytest.mark.parametrize("room", ["none", "short", "odd", "right"])
+def test_grouped_workspace(room):
+    """With any workspace, or none that can be used, the same bits; rows behind the groups may hold any index."""
+    e, k, m, n = 2, 272, 130, 50
+    counts = [70, 41]
+    c, o = tables(counts)
+    w, ws, x, xs = operands(3, n, k, m, e)
+    rows = torch.randint(0, 3 * n, (120,), generator=gen(9), device="cuda", dtype=torch.int32)
+    rows[111:] = torch.tensor([-1, -2 ** 31, 2 ** 31 - 1, 3 * n, 0, 1, 2, 3, 4], dtype=torch.int32, device="cuda")
+    need = ops.mul_mat_f8_grouped_workspace(k, 120, e)
+    assert need > 0 and ops.mul_mat_f8_grouped_workspace(k, 16 * e, e) == 0
+    work = {"none": torch.empty(0, dtype=torch.uint8, device="cuda"), "short": torch.empty(need - 1, dtype=torch.uint8, device="cuda"),
+            "odd": torch.empty(need + 1, dtype=torch.uint8, device="cuda")[1:], "right": torch.empty(need, dtype=torch.uint8, device="cuda")}
+    out = torch.full((120, m), 5.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = ops.mul_mat_f8_grouped(w, ws, x, xs, c, o, rows=rows, n_selected=3, out=out, workspace=work[room], status=status)
+    check_grouped(got, w, ws, x, xs, counts, o.tolist(), (rows // 3).long(), k)
+    assert torch.all(got[111:] == 5.0) and int(status) == 0
+    assert torch.equal(got[:111], ops.mul_mat_f8_grouped(w, ws, x, xs, c, o, rows=rows, n_selected=3)[:111])
+
+
 def test_grouped_many_experts():
     e, k, m = 300, 128, 48
     g = gen(1)
@@ -421,6 +442,16 @@ def test_grouped_bad_tables(k, m):
     out.fill_(5.0)
     ops.mul_mat_f8_grouped(w, ws, x, xs, c, o, rows=rows, out=out)  # no status word
     assert torch.all(out[1:4] == 0)
+    # the same where the rows are copied first
+    many = torch.arange(100, dtype=torch.int32, device="cuda") % 40
+    many[1], many[2], many[3] = -1, 40, 2 ** 31 - 1
+    c, o = tables([90, 0, 0, 0])
+    big = torch.full((100, m), 5.0, device="cuda")
+    status.zero_()
+    ops.mul_mat_f8_grouped(w, ws, x, xs, c, o, rows=many, out=big, status=status)
+    good = torch.tensor([0] + list(range(4, 90)), device="cuda")
+    check_product(big[good], *product64(w[0], ws[0], x[many[good].long()], xs[many[good].long()]), k)
+    assert torch.all(big[1:4] == 0) and torch.all(big[90:] == 5.0) and int(status) == 2
 
 
 # ---------------------------------------------------------------------------------------------------------------
