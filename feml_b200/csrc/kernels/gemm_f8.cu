@@ -39,6 +39,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../host_common.h"
 #include "gemm_f8.cuh"
@@ -50,19 +51,16 @@ namespace fbk {
 namespace {
 
 constexpr int GM = 128;           // rows per tile
-#ifndef G_EPI_WARPS_
-#define G_EPI_WARPS_ 8
-#endif
-constexpr int G_EPI_WARPS = G_EPI_WARPS_;
+constexpr int G_EPI_WARPS = 8;
 constexpr int G_EPI_GROUPS = G_EPI_WARPS / 4;
 constexpr int G_THREADS = 128 + 32 * G_EPI_WARPS;
 constexpr int G_XBOX = 32;        // rows per TMA box of x: only boxes with live rows are fetched
 constexpr int G_MAX_E = 1024;
-constexpr int G_REGS_EPI = G_EPI_WARPS == 8 ? 208 : 104, G_REGS_REST = G_EPI_WARPS == 8 ? 88 : 64;
+constexpr int G_REGS_EPI = 208, G_REGS_REST = 88;
 constexpr int G_SCB = 8;          // blocks per chunk of scales
 constexpr int G_SCR = 3;          // chunks in flight
 constexpr int G_SCP = GM + 4;     // floats between two blocks of a chunk (the copy to it has no bank conflicts)
-constexpr int G_STG = 32;         // bytes of a row that an epilogue warp stages at a time
+constexpr int G_STG = 64;         // bytes of a row that an epilogue warp stages at a time
 
 template <int BN>
 struct GCfg {
@@ -77,7 +75,7 @@ struct GCfg {
     static constexpr int OFF_SX = OFF_GRP + (G_MAX_E + 1) * 4 + 12;
     static constexpr int OFF_SW = OFF_SX + G_SCR * G_SCB * G_SCP * 4;
     static constexpr int OFF_BAR = OFF_SW + G_SCR * G_SCB * 2 * 4;
-    static constexpr int BYTES = OFF_BAR + (2 * NS + 2 * NB + 2 * G_SCR + 1) * 8 + 16 + 1024;
+    static constexpr int BYTES = OFF_BAR + (2 * NS + NB + 2 * G_SCR + 1) * 8 + 16 + 1024;
     static_assert(OFF_BAR % 8 == 0 && BYTES <= 232448, "shared memory");
     static_assert(GM * (BN + 4) * 4 <= NS * STAGE, "partial tile of a split");
 };
@@ -104,6 +102,19 @@ __device__ __forceinline__ void mma_f8f6f4(uint32_t d, uint64_t adesc, uint64_t 
 
 // Instruction descriptor, kind::f8f6f4: D f32, A and B e4m3, both K-major.
 constexpr uint32_t f8_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+
+// c += a * b in c's own registers.
+__device__ __forceinline__ void f2_fma_in_place(uint64_t &c, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+
+// A TMEM buffer is free again: the epilogue warps arrive, the MMA warp waits.
+__device__ __forceinline__ void buf_arrive(int u) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(2 + u), "n"(32 * (G_EPI_WARPS + 1)) : "memory");
+}
+__device__ __forceinline__ void buf_wait(int u) {
+    asm volatile("bar.sync %0, %1;" ::"r"(2 + u), "n"(32 * (G_EPI_WARPS + 1)) : "memory");
+}
 
 // The gate warp and the epilogue warps meet once per block.
 __device__ __forceinline__ void gate_sync() {
@@ -204,40 +215,71 @@ __device__ __forceinline__ void store16(uint8_t *row, int m, int M, uint4 v, boo
     }
 }
 
-// One warp's 32 rows x COLS columns of finished sums (a row per lane): 32
-// bytes of each row at a time through 1 KB of shared memory, so that the
-// global stores cover whole sectors. 16-byte unit u of row r lies at
-// u ^ ((r >> 2) & 1): neither side has bank conflicts.
+// Columns c, c + 1, ... of a row's sums as 16 bytes of output.
+template <typename T>
+__device__ __forceinline__ uint4 pack_sums(const uint64_t *acc) {
+    if constexpr (sizeof(T) == 4)
+        return make_uint4((uint32_t)acc[0], (uint32_t)(acc[0] >> 32), (uint32_t)acc[1], (uint32_t)(acc[1] >> 32));
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float x, y;
+        f2_unpack(acc[sizeof(T) == 4 ? 0 : i], x, y);
+        w[i] = pack2<typename std::conditional<sizeof(T) == 4, __half, T>::type>(x, y);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+
+// One warp's 32 rows x COLS columns of finished sums (a row per lane): 64
+// bytes of each row at a time through 2 KB of shared memory, so that a store
+// instruction covers 64 bytes of 8 rows instead of 16 bytes of 32. 16-byte
+// unit u of row r lies at u ^ ((r >> 1) & 3): neither side has bank conflicts.
+// `out`: the warp's first row; rows in `bad` become zeros. A whole aligned
+// tile stores through four row pointers and immediate offsets: with the edge
+// checks in its way the output took 15% of a tile's time (K = 4096).
 template <typename T, int COLS>
-__device__ __forceinline__ void store_rows(const float (&acc)[COLS], uint32_t stage, const GTile &t, int r_first, int m0,
-                                           const F8Gemm &p, int lane, bool wide) {
-    constexpr int N = Vec<T>::N;
+__device__ __forceinline__ void store_rows(const uint64_t (&acc)[COLS / 2], uint32_t stage, uint8_t *out, uint64_t nb1, int rows,
+                                           int m0, int M, uint32_t bad, int lane, bool wide) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const int r0 = lane >> 2, u0 = lane & 3;
+    const uint32_t to = stage + lane * G_STG, from = stage + r0 * G_STG + ((u0 ^ ((r0 >> 1) & 3)) << 4);
+    const uint32_t sw = (lane >> 1) & 3;
+    const bool whole = wide && rows >= 32 && m0 + COLS <= M && bad == 0;
+    uint8_t *o[4];
 #pragma unroll
-    for (int c = 0; c < COLS; c += 2 * N) {
+    for (int i = 0; i < 4; i++) o[i] = out + (uint64_t)(i * 8 + r0) * nb1 + (uint64_t)(m0 + u0 * N) * sizeof(T);
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const uint4 v = pack16<T>(&acc[c + u * N]);
-            const uint32_t a = stage + lane * G_STG + ((u ^ ((lane >> 2) & 1)) << 4);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-        }
+    for (int c = 0; c < COLS; c += 4 * N) {
+#pragma unroll
+        for (uint32_t u = 0; u < 4; u++) sts16(to + ((u ^ sw) << 4), pack_sums<T>(&acc[(c + u * N) / 2]));
         __syncwarp();
+        uint4 v[4];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int r = i * 16 + (lane >> 1), u = lane & 1;
-            uint4 v;
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                         : "r"(stage + r * G_STG + ((u ^ ((r >> 2) & 1)) << 4))
-                         : "memory");
-            const int m = m0 + c + u * N;
-            if (r_first + r < t.rows && m < p.M)
-                store16<T>(p.y + (uint64_t)(t.row0 + r_first + r) * p.y_nb1, m, p.M, v, wide);
+        for (int i = 0; i < 4; i++) v[i] = lds16(from + i * 8 * G_STG);
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(o[i] + c * sizeof(T)) = v[i];
+        } else {
+            const int m = m0 + c + u0 * N;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (bad >> (i * 8 + r0) & 1) v[i] = make_uint4(0, 0, 0, 0);
+                if (i * 8 + r0 < rows && m < M) store16<T>(out + (uint64_t)(i * 8 + r0) * nb1, m, M, v[i], wide);
+            }
         }
         __syncwarp();
     }
 }
 
-template <int BN, bool SPLIT, bool GATHER>
+template <int BN, bool SPLIT, bool GATHER, typename T>
 __global__ void __launch_bounds__(G_THREADS, 1)
     gemm_f8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                    const __grid_constant__ GParams q) {
@@ -249,8 +291,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     uint64_t *full = reinterpret_cast<uint64_t *>(gbase + C::OFF_BAR);
     uint64_t *empty = full + C::NS;
     uint64_t *t_full = empty + C::NS;
-    uint64_t *t_empty = t_full + C::NB;
-    uint64_t *s_full = t_empty + C::NB;
+    uint64_t *s_full = t_full + C::NB;
     uint64_t *s_empty = s_full + G_SCR;
     uint64_t *drained = s_empty + G_SCR;
     float *sx = reinterpret_cast<float *>(gbase + C::OFF_SX);
@@ -265,10 +306,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < C::NB; i++) {
-            mbar_init(&t_full[i], 1);
-            mbar_init(&t_empty[i], G_EPI_WARPS);
-        }
+        for (int i = 0; i < C::NB; i++) mbar_init(&t_full[i], 1);
         for (int i = 0; i < G_SCR; i++) {
             mbar_init(&s_full[i], 32);
             mbar_init(&s_empty[i], G_EPI_WARPS);
@@ -352,15 +390,13 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             const uint64_t desc0 = sw128_desc(sbase);
             int it = 0;
             bool ok = true;
-            for (int t = t0; ok; t += t_step) {
+            for (int t = t0;; t += t_step) {
                 if (g_tile(q, start, t, BN).expert < 0) break;
                 for (int b = b0; b < b1; b++, it++) {
                     const int s = it % C::NS, u = it % C::NB;
-                    if (!tc_wait_all(&full[s], (it / C::NS) & 1, abort_flag) ||
-                        !tc_wait_all(&t_empty[u], ((it / C::NB) & 1) ^ 1, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = ok && tc_wait_all(&full[s], (it / C::NS) & 1, abort_flag);
+                    if (it >= C::NB) buf_wait(u);
+                    if (!ok) continue;  // (after an abort: the handshakes only)
                     tc_fence_after();
                     const uint64_t xd = desc0 + (uint64_t)(s * (C::STAGE / 16)), wd = xd + C::X_STAGE / 16;
                     const uint32_t d = tmem + (uint32_t)(u * BN);
@@ -374,6 +410,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                 }
             }
             if (elect_one()) tc_commit(smem_u32(drained));  // every MMA issued here
+            for (int i = max(0, it - C::NB); i < it; i++) buf_wait(i % C::NB);
         } else if (warp == 2) {
             // ---- scales: G_SCB blocks of 128 rows at a time, eight lanes per row -------------
             const int j = lane & 7;
@@ -439,67 +476,68 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         const uint32_t stage = sbase + C::OFF_OUT + ew * 32 * G_STG;
         int it = 0, ch = 0;
         for (int t = t0;; t += t_step) {
-            const GTile tile = g_tile(q, start, t, BN);
-            if (tile.expert < 0) break;
+            if (g_tile(q, start, t, BN).expert < 0) break;
             const int r_first = part * 32, row = r_first + lane;
-            const bool any = r_first < tile.rows;  // (warp-uniform)
             uint64_t acc[C::COLS / 2];
 #pragma unroll
             for (int i = 0; i < C::COLS / 2; i++) acc[i] = 0;
+            float sc = 0.0f;
+#pragma unroll 1
             for (int b = b0; b < b1; b++, it++) {
                 const int u = it % C::NB, j = (b - b0) % G_SCB, c = ch % G_SCR;
                 gate_sync();
-                // a warpgroup's columns lie in one block row of the weights
-                const float sc = sx[(c * G_SCB + j) * G_SCP + row] * sw[(c * G_SCB + j) * 2 + grp * C::COLS / F8B];
-                if (any) {
+                // a warpgroup's columns lie in one block row of the weights; the
+                // scales of the next block are read behind this block's loads
+                const float *sxc = &sx[c * G_SCB * G_SCP + row], *swc = &sw[c * G_SCB * 2 + grp * C::COLS / F8B];
+                if (j == 0) sc = sxc[0] * swc[0];
+                {
                     tc_fence_after();
                     const uint64_t sc2 = f2_pack(sc, sc);
                     uint32_t v[2][16];
                     tc_ld16(lanes + (uint32_t)(u * BN), v[0]);
+                    const int jn = j + 1 < G_SCB ? j + 1 : 0;
+                    sc = sxc[jn * G_SCP] * swc[jn * 2];
                     tc_wait_ld();
 #pragma unroll
                     for (int h = 0; h < C::COLS / 16; h++) {
                         if (h + 1 < C::COLS / 16) tc_ld16(lanes + (uint32_t)(u * BN + (h + 1) * 16), v[(h + 1) & 1]);
 #pragma unroll
                         for (int i = 0; i < 8; i++)
-                            acc[h * 8 + i] = f2_fma(f2_pack_bits(v[h & 1][2 * i], v[h & 1][2 * i + 1]), sc2, acc[h * 8 + i]);
+                            f2_fma_in_place(acc[h * 8 + i], f2_pack_bits(v[h & 1][2 * i], v[h & 1][2 * i + 1]), sc2);
                         if (h + 1 < C::COLS / 16) tc_wait_ld();
+                        if (h + 2 == C::COLS / 16) {  // all of it is in registers
+                            tc_fence_before();
+                            buf_arrive(u);
+                        }
                     }
-                    tc_fence_before();
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&t_empty[u]);
                 if (j == G_SCB - 1 || b == b1 - 1) {
+                    __syncwarp();
                     if (lane == 0) mbar_arrive(&s_empty[c]);
                     ch++;
                 }
             }
+            // (the tile again: kept across the loop it costs the accumulators' registers)
+            int t2 = t;
+            asm volatile("" : "+r"(t2));
+            const GTile tile = g_tile(q, start, t2, BN);
             int src = -1;
             if (row < tile.rows) src = p.g.counts ? f8_origin(p.g, tile.row0 + row, p.status) : 0;
-            float f[C::COLS];
-#pragma unroll
-            for (int i = 0; i < C::COLS / 2; i++) f2_unpack(acc[i], f[2 * i], f[2 * i + 1]);
-            if (src < 0) {
-#pragma unroll
-                for (int i = 0; i < C::COLS; i++) f[i] = 0.0f;
-            }
             if constexpr (SPLIT) {
                 // the pipeline's stages are free: every copy was consumed and every MMA has been read
                 float *mine = reinterpret_cast<float *>(gbase) + row * (BN + 4) + grp * C::COLS;
                 if (row < tile.rows) {
 #pragma unroll
-                    for (int i = 0; i < C::COLS; i += 4)
-                        *reinterpret_cast<float4 *>(mine + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                    for (int i = 0; i < C::COLS / 2; i += 2)
+                        *reinterpret_cast<ulonglong2 *>(mine + 2 * i) = make_ulonglong2(src >= 0 ? acc[i] : 0, src >= 0 ? acc[i + 1] : 0);
                 }
-            } else if (any && !*abort_flag) {
-                const int m0 = tile.m0 + grp * C::COLS;
+            } else {
+                const uint32_t bad = __ballot_sync(0xffffffffu, src < 0);
                 const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | p.y_nb1) & 15) == 0;
-                if (p.out_type == FB_F32)
-                    store_rows<float, C::COLS>(f, stage, tile, r_first, m0, p, lane, wide);
-                else if (p.out_type == FB_F16)
-                    store_rows<__half, C::COLS>(f, stage, tile, r_first, m0, p, lane, wide);
-                else
-                    store_rows<__nv_bfloat16, C::COLS>(f, stage, tile, r_first, m0, p, lane, wide);
+                const int rows = tile.rows - r_first;
+                if (rows > 0 && !*abort_flag)
+                    store_rows<T, C::COLS>(acc, stage, p.y + (uint64_t)(tile.row0 + r_first) * p.y_nb1, p.y_nb1, rows,
+                                           tile.m0 + grp * C::COLS, p.M, bad, lane, wide);
             }
         }
     }
@@ -524,14 +562,8 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                     const int m = tile.m0 + c;
                     uint8_t *o = p.y + (uint64_t)(tile.row0 + r) * p.y_nb1;
                     if (m < p.M) {
-                        if (p.out_type == FB_F32) {
-                            store16<float>(o, m, p.M, pack16<float>(f), wide);
-                            if (m + 4 < p.M) store16<float>(o, m + 4, p.M, pack16<float>(f + 4), wide);
-                        } else if (p.out_type == FB_F16) {
-                            store16<__half>(o, m, p.M, pack16<__half>(f), wide);
-                        } else {
-                            store16<__nv_bfloat16>(o, m, p.M, pack16<__nv_bfloat16>(f), wide);
-                        }
+                        store16<T>(o, m, p.M, pack16<T>(f), wide);
+                        if (sizeof(T) == 4 && m + 4 < p.M) store16<T>(o, m + 4, p.M, pack16<T>(f + 8 - Vec<T>::N), wide);
                     }
                 }
             }
@@ -567,17 +599,17 @@ __global__ void __launch_bounds__(256) gather_f8_kernel(const F8Gemm p, uint8_t 
     for (int b = lane; b < kb; b += 32) sg[(int64_t)r * kb + b] = s[b];
 }
 
-template <int BN, bool SPLIT, bool GATHER>
+template <int BN, bool SPLIT, bool GATHER, typename T>
 int launch_t(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const GParams &q, int ctas, int cluster, cudaStream_t s) {
     using C = GCfg<BN>;
-    auto *fn = gemm_f8_kernel<BN, SPLIT, GATHER>;
+    auto *fn = gemm_f8_kernel<BN, SPLIT, GATHER, T>;
     static DeviceFlags done;
     int rc = raise_smem_limit(reinterpret_cast<const void *>(fn), C::BYTES, done, "mul_mat_f8");
     if (rc) return rc;
     // setmaxnreg draws on the registers of the launch: the two shares must fit
     static const int regs = [] {
         cudaFuncAttributes a{};
-        return cudaFuncGetAttributes(&a, reinterpret_cast<const void *>(gemm_f8_kernel<BN, SPLIT, GATHER>)) == cudaSuccess ? a.numRegs : 0;
+        return cudaFuncGetAttributes(&a, reinterpret_cast<const void *>(gemm_f8_kernel<BN, SPLIT, GATHER, T>)) == cudaSuccess ? a.numRegs : 0;
     }();
     if (regs * G_THREADS < 32 * G_EPI_WARPS * G_REGS_EPI + 128 * G_REGS_REST)
         return fb::set_error(FB_ERR_CUDA, "mul_mat_f8: built with %d registers per thread", regs);
@@ -597,11 +629,18 @@ int launch_t(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const GParams &q,
     return FB_OK;
 }
 
+template <int BN, bool SPLIT, bool GATHER>
+int launch_o(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const GParams &q, int ctas, int cluster, cudaStream_t s) {
+    if (q.p.out_type == FB_F32) return launch_t<BN, SPLIT, GATHER, float>(tm_w, tm_x, q, ctas, cluster, s);
+    if (q.p.out_type == FB_F16) return launch_t<BN, SPLIT, GATHER, __half>(tm_w, tm_x, q, ctas, cluster, s);
+    return launch_t<BN, SPLIT, GATHER, __nv_bfloat16>(tm_w, tm_x, q, ctas, cluster, s);
+}
+
 template <int BN, bool SPLIT>
 int launch_g(bool gather, const CUtensorMap &tm_w, const CUtensorMap &tm_x, const GParams &q, int ctas, int cluster,
              cudaStream_t s) {
-    return gather ? launch_t<BN, SPLIT, true>(tm_w, tm_x, q, ctas, cluster, s)
-                  : launch_t<BN, SPLIT, false>(tm_w, tm_x, q, ctas, cluster, s);
+    return gather ? launch_o<BN, SPLIT, true>(tm_w, tm_x, q, ctas, cluster, s)
+                  : launch_o<BN, SPLIT, false>(tm_w, tm_x, q, ctas, cluster, s);
 }
 
 }  // namespace
