@@ -301,6 +301,10 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const F8Gemm &p = q.p;
 
+    if (tid == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_x) : "memory");
+    }
     if (tid == 0) {
         for (int i = 0; i < C::NS; i++) {
             mbar_init(&full[i], 1);
@@ -320,6 +324,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // (up to here no global memory: the set-up overlaps the end of the stream's previous kernel)
+    grid_dependency_wait();
+    grid_launch_dependents();
     if (warp == 3 && p.g.counts) {  // first tile of every group
         int run = 0;
         for (int e0 = 0; e0 < p.g.n_experts; e0 += 32) {
@@ -583,6 +590,8 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 // Gathered copies: a warp per row. A row whose table entry is out of range is
 // left as it is: the product checks the table again and writes zeros.
 __global__ void __launch_bounds__(256) gather_f8_kernel(const F8Gemm p, uint8_t *xg, uint64_t xg_nb1, float *sg, int kb) {
+    grid_dependency_wait();
+    grid_launch_dependents();
     const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (r >= p.g.n_rows) return;
     const int src = f8_source(p.g, r, nullptr);
@@ -613,20 +622,8 @@ int launch_t(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const GParams &q,
     }();
     if (regs * G_THREADS < 32 * G_EPI_WARPS * G_REGS_EPI + 128 * G_REGS_REST)
         return fb::set_error(FB_ERR_CUDA, "mul_mat_f8: built with %d registers per thread", regs);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(G_THREADS);
-    cfg.dynamicSmemBytes = C::BYTES;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = SPLIT ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tm_w, tm_x, q);
-    if (e != cudaSuccess) return fb::set_error(FB_ERR_CUDA, "mul_mat_f8 launch: %s", cudaGetErrorString(e));
-    return FB_OK;
+    return launch_early("mul_mat_f8", gemm_f8_kernel<BN, SPLIT, GATHER, T>, dim3((unsigned)ctas), dim3(G_THREADS), C::BYTES, cluster, s,
+                        tm_w, tm_x, q);
 }
 
 template <int BN, bool SPLIT, bool GATHER>
@@ -667,9 +664,9 @@ int launch_gather_f8(F8Gemm &p, void *ws, cudaStream_t s) {
     uint8_t *xg = static_cast<uint8_t *>(ws);
     float *sg = reinterpret_cast<float *>(xg + (uint64_t)p.g.n_rows * nb1);
     const int kb = (p.K + F8B - 1) / F8B;
-    gather_f8_kernel<<<(unsigned)(((int64_t)p.g.n_rows + 7) / 8), 256, 0, s>>>(p, xg, nb1, sg, kb);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fb::set_error(FB_ERR_CUDA, "mul_mat_f8_grouped launch: %s", cudaGetErrorString(e));
+    const int rc = launch_early("mul_mat_f8_grouped", gather_f8_kernel, dim3((unsigned)(((int64_t)p.g.n_rows + 7) / 8)), dim3(256), 0, 1,
+                                s, p, xg, nb1, sg, kb);
+    if (rc) return rc;
     p.x = xg;
     p.x_nb1 = nb1;
     p.xs = reinterpret_cast<const uint8_t *>(sg);

@@ -32,6 +32,8 @@ __global__ void __launch_bounds__(A_THREADS) gemm_f8_any_kernel(const F8Gemm p) 
     __shared__ __align__(16) uint8_t sx[AB * A_PITCH], sw[AB * A_PITCH];
     __shared__ int src[AB];
     __shared__ F8Group s_grp;
+    grid_dependency_wait();
+    grid_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int m0 = blockIdx.y * AB;
     F8Group grp{0, (int)blockIdx.x * AB, 0};
@@ -125,15 +127,10 @@ int launch_gemm_f8_any(const F8Gemm &p, cudaStream_t s) {
     const int64_t gy = ((int64_t)p.M + AB - 1) / AB;
     if (gy > 65535) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: %d rows of unaligned weights", p.M);
     const dim3 grid((unsigned)gx, (unsigned)gy);
-    if (p.out_type == FB_F32)
-        gemm_f8_any_kernel<float><<<grid, A_THREADS, 0, s>>>(p);
-    else if (p.out_type == FB_F16)
-        gemm_f8_any_kernel<__half><<<grid, A_THREADS, 0, s>>>(p);
-    else
-        gemm_f8_any_kernel<__nv_bfloat16><<<grid, A_THREADS, 0, s>>>(p);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fb::set_error(FB_ERR_CUDA, "mul_mat_f8 launch: %s", cudaGetErrorString(e));
-    return FB_OK;
+    const char *what = "mul_mat_f8";
+    if (p.out_type == FB_F32) return launch_early(what, gemm_f8_any_kernel<float>, grid, dim3(A_THREADS), 0, 1, s, p);
+    if (p.out_type == FB_F16) return launch_early(what, gemm_f8_any_kernel<__half>, grid, dim3(A_THREADS), 0, 1, s, p);
+    return launch_early(what, gemm_f8_any_kernel<__nv_bfloat16>, grid, dim3(A_THREADS), 0, 1, s, p);
 }
 
 }  // namespace fbk

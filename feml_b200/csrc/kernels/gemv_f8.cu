@@ -189,21 +189,7 @@ __global__ void __launch_bounds__(32 * V_WARPS) gemv_f8_kernel(const F8Gemm p, i
 
 template <int NT, typename T>
 int launch_v(const F8Gemm &p, int ctas, int splits, cudaStream_t s) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(32 * V_WARPS);
-    cfg.stream = s;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = (unsigned)splits;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = splits > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemv_f8_kernel<NT, T>, p, splits);
-    if (e != cudaSuccess) return fb::set_error(FB_ERR_CUDA, "mul_mat_f8 launch: %s", cudaGetErrorString(e));
-    return FB_OK;
+    return launch_early("mul_mat_f8", gemv_f8_kernel<NT, T>, dim3((unsigned)ctas), dim3(32 * V_WARPS), 0, splits, s, p, splits);
 }
 
 }  // namespace

@@ -225,6 +225,33 @@ int launch_silu_f32(const void *x, const uint64_t *xnb, void *y, const uint64_t 
                     cudaStream_t s);
 int launch_bias_act(void *y, uint64_t y_nb1, int64_t M, int64_t N, const EpiAct &epi, cudaStream_t s);
 
+// Launch that may begin while the stream's previous kernel ends (programmatic
+// dependent launch); `cluster` CTAs per cluster when above 1. Every kernel
+// launched so calls grid_dependency_wait() in all threads before it touches
+// global memory, so the order of the stream's results is kept.
+#ifdef __CUDACC__
+template <typename... P, typename... A>
+inline int launch_early(const char *what, void (*fn)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t s,
+                        const A &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, args...);
+    if (e != cudaSuccess) return fb::set_error(FB_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+    return FB_OK;
+}
+#endif
+
 // ---- e4m3 operators (f8.cuh: values, scales) --------------------------------
 // Where a row operator writes: q row r at q + r*q_nb1 (one byte per value),
 // its scales (one f32 per 128 values, or per 128 x 128 block) at scale +

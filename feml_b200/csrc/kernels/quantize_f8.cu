@@ -47,6 +47,8 @@ __device__ __forceinline__ float silu_mul_f(float g, float u) { return __fdivide
 
 template <typename T, bool SILU, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) rows_f8_kernel(const RowParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
     constexpr int N = VEC ? Vec<T>::N : 4;
     constexpr int G = F8B / N;
     const int lane = threadIdx.x % G;
@@ -145,6 +147,8 @@ __global__ void __launch_bounds__(kTileThreads) tile_f8_kernel(const TileParams 
     constexpr int RS = kTileThreads / G;        // rows per step
     constexpr int STEPS = F8B / RS;
     __shared__ uint32_t s_top[kTileThreads / 32];
+    grid_dependency_wait();
+    grid_launch_dependents();
     const int64_t br = blockIdx.x / p.kb;
     const uint32_t bc = (uint32_t)(blockIdx.x - br * p.kb);
     const int64_t k = (int64_t)bc * F8B + (threadIdx.x % G) * N;
@@ -237,6 +241,8 @@ template <typename T, int NV, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8Params p) {
     constexpr int N = Vec<T>::N, G = F8B / N;
     __shared__ float part[32];
+    grid_dependency_wait();
+    grid_launch_dependents();
     const int64_t row = WARP ? (int64_t)blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
     if (WARP && row >= p.rows) return;
     const int t = threadIdx.x, nt = WARP ? 32 : blockDim.x;
@@ -329,6 +335,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_f8_any_kernel(const NormF8Params p) {
     __shared__ float part[32];
+    grid_dependency_wait();
+    grid_launch_dependents();
     const int64_t row = blockIdx.x;
     const T *x = reinterpret_cast<const T *>(p.x + row * p.x_nb1);
     const T *res = p.res ? reinterpret_cast<const T *>(p.res + row * p.res_nb1) : nullptr;
@@ -374,12 +382,6 @@ __global__ void __launch_bounds__(1024) norm_f8_any_kernel(const NormF8Params p)
     }
 }
 
-int launched(const char *what) {
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fb::set_error(FB_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
-    return FB_OK;
-}
-
 bool aligned(uint64_t a, const void *p, uint64_t nb1) { return ((reinterpret_cast<uintptr_t>(p) | nb1) & (a - 1)) == 0; }
 
 template <typename T, bool SILU>
@@ -387,21 +389,18 @@ int launch_rows_t(const RowParams &p, bool vec, cudaStream_t s, const char *what
     const int groups = kRowThreads / (vec ? F8B / Vec<T>::N : 32);
     const int64_t grid = (p.total + groups - 1) / groups;
     if (grid > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "%s: too many blocks", what);
-    if (vec)
-        rows_f8_kernel<T, SILU, true><<<(unsigned)grid, kRowThreads, 0, s>>>(p);
-    else
-        rows_f8_kernel<T, SILU, false><<<(unsigned)grid, kRowThreads, 0, s>>>(p);
-    return launched(what);
+    return launch_early(what, vec ? rows_f8_kernel<T, SILU, true> : rows_f8_kernel<T, SILU, false>, dim3((unsigned)grid),
+                        dim3(kRowThreads), 0, 1, s, p);
 }
 
 template <typename T>
 int launch_norm_t(const NormF8Params &p, bool vec, cudaStream_t s) {
+    const char *what = "rms_norm_f8";
     constexpr int N = Vec<T>::N;
     const int64_t vecs = p.k / N;
     if (!vec || vecs > 8 * 1024) {
         const int threads = (int)std::min<int64_t>(1024, (p.k + 31) / 32 * 32);
-        norm_f8_any_kernel<T><<<(unsigned)p.rows, threads, 0, s>>>(p);
-        return launched("rms_norm_f8");
+        return launch_early(what, norm_f8_any_kernel<T>, dim3((unsigned)p.rows), dim3(threads), 0, 1, s, p);
     }
     // A warp per row for short rows in numbers that fill the GPU; else a CTA
     // per row: one vector per thread when rows are few (latency), more
@@ -409,28 +408,19 @@ int launch_norm_t(const NormF8Params &p, bool vec, cudaStream_t s) {
     if (vecs <= 128 && p.rows >= 1024) {
         const dim3 block(32, 8);
         const unsigned grid = (unsigned)((p.rows + 7) / 8);
-        if (vecs <= 32)
-            norm_f8_kernel<T, 1, true><<<grid, block, 0, s>>>(p);
-        else if (vecs <= 64)
-            norm_f8_kernel<T, 2, true><<<grid, block, 0, s>>>(p);
-        else
-            norm_f8_kernel<T, 4, true><<<grid, block, 0, s>>>(p);
-        return launched("rms_norm_f8");
+        auto *fn = vecs <= 32 ? norm_f8_kernel<T, 1, true> : vecs <= 64 ? norm_f8_kernel<T, 2, true> : norm_f8_kernel<T, 4, true>;
+        return launch_early(what, fn, dim3(grid), block, 0, 1, s, p);
     }
     const int most = p.rows <= 296 ? 1024 : 256;
     int nv = 1;
     while (nv < 8 && (vecs + nv - 1) / nv > most) nv *= 2;
     const int threads = (int)(((vecs + nv - 1) / nv + 31) / 32 * 32);
     const unsigned grid = (unsigned)p.rows;
-    if (nv == 1)
-        norm_f8_kernel<T, 1, false><<<grid, threads, 0, s>>>(p);
-    else if (nv == 2)
-        norm_f8_kernel<T, 2, false><<<grid, threads, 0, s>>>(p);
-    else if (nv == 4)
-        norm_f8_kernel<T, 4, false><<<grid, threads, 0, s>>>(p);
-    else
-        norm_f8_kernel<T, 8, false><<<grid, threads, 0, s>>>(p);
-    return launched("rms_norm_f8");
+    auto *fn = nv == 1   ? norm_f8_kernel<T, 1, false>
+               : nv == 2 ? norm_f8_kernel<T, 2, false>
+               : nv == 4 ? norm_f8_kernel<T, 4, false>
+                         : norm_f8_kernel<T, 8, false>;
+    return launch_early(what, fn, dim3(grid), dim3(threads), 0, 1, s, p);
 }
 
 int esize(int32_t type) { return type == FB_F32 ? 4 : 2; }
@@ -481,21 +471,10 @@ int launch_quantize_f8_tiles(int32_t type, const void *x, uint64_t x_nb1, int64_
     if (grid > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "quantize_f8: too many blocks");
     const int n = 16 / esize(type);
     const bool vec = k % n == 0 && aligned(16, x, x_nb1) && aligned(n, o.q, o.q_nb1);
-    const unsigned g = (unsigned)grid;
-#define FB_TILE(T)                                            \
-    if (vec)                                                  \
-        tile_f8_kernel<T, true><<<g, kTileThreads, 0, s>>>(p); \
-    else                                                      \
-        tile_f8_kernel<T, false><<<g, kTileThreads, 0, s>>>(p);
-    if (type == FB_F32) {
-        FB_TILE(float)
-    } else if (type == FB_F16) {
-        FB_TILE(__half)
-    } else {
-        FB_TILE(__nv_bfloat16)
-    }
-#undef FB_TILE
-    return launched("quantize_f8");
+    auto *fn = type == FB_F32   ? (vec ? tile_f8_kernel<float, true> : tile_f8_kernel<float, false>)
+               : type == FB_F16 ? (vec ? tile_f8_kernel<__half, true> : tile_f8_kernel<__half, false>)
+                                : (vec ? tile_f8_kernel<__nv_bfloat16, true> : tile_f8_kernel<__nv_bfloat16, false>);
+    return launch_early("quantize_f8", fn, dim3((unsigned)grid), dim3(kTileThreads), 0, 1, s, p);
 }
 
 int launch_rms_norm_f8(int32_t type, const void *x, uint64_t x_nb1, const void *residual, uint64_t residual_nb1,
