@@ -37,6 +37,7 @@ struct RowParams {
     int64_t total;  // rows * blocks per row
     int64_t k;
     uint32_t kb;    // blocks per row
+    uint32_t kb_mul, kb_shift;  // n / kb = (mulhi(n, kb_mul) + n) >> kb_shift, n < 2^31
 };
 
 // silu(g) * u = g / (1 + e^-g) * u. The exponential and the division are the
@@ -54,11 +55,12 @@ __global__ void __launch_bounds__(kRowThreads) rows_f8_kernel(const RowParams p)
     const int lane = threadIdx.x % G;
     const int64_t gid = (int64_t)blockIdx.x * (kRowThreads / G) + threadIdx.x / G;
     const bool live = gid < p.total;
-    // one division by the blocks per row, in 32 bits where the count allows
+    // the division by the blocks per row: by a multiplication where the count
+    // fits 31 bits
     int64_t row;
     uint32_t b;
     if (p.total <= 0x7fffffff) {
-        row = (uint32_t)gid / p.kb;
+        row = (__umulhi((uint32_t)gid, p.kb_mul) + (uint32_t)gid) >> p.kb_shift;
         b = (uint32_t)gid - (uint32_t)row * p.kb;
     } else {
         row = gid / p.kb;
@@ -442,6 +444,8 @@ int launch_rows_f8(int32_t type, const void *x, uint64_t x_nb1, const void *up, 
     p.k = k;
     p.kb = (uint32_t)((k + F8B - 1) / F8B);
     p.total = rows * p.kb;
+    while ((1ull << p.kb_shift) < p.kb) p.kb_shift++;
+    p.kb_mul = (uint32_t)(((1ull << 32) * ((1ull << p.kb_shift) - p.kb)) / p.kb + 1);
     const int n = 16 / esize(type);
     const bool vec = k % n == 0 && aligned(16, x, x_nb1) && (!up || aligned(16, up, up_nb1)) && aligned(n, o.q, o.q_nb1);
     switch (type) {
