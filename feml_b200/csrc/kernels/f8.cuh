@@ -110,6 +110,18 @@ __device__ __forceinline__ uint4 ld_stream16(const void *p) {
     return v;
 }
 
+struct alignas(32) Wide32 {
+    uint4 lo, hi;
+};
+// The same for 32 bytes in one instruction.
+__device__ __forceinline__ Wide32 ld_stream32(const void *p) {
+    Wide32 v;
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v.lo.x), "=r"(v.lo.y), "=r"(v.lo.z), "=r"(v.lo.w), "=r"(v.hi.x), "=r"(v.hi.y), "=r"(v.hi.z), "=r"(v.hi.w)
+                 : "l"(p));
+    return v;
+}
+
 // Magnitudes compare as integers: every NaN is above infinity, infinity above
 // every finite value, so an integer maximum carries a NaN along.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }

@@ -20,10 +20,12 @@ namespace {
 
 // ---------------------------------------------------------------------------
 // quantize (one operand) and silu_mul (two): blocks are independent. A block
-// of 128 values belongs to G consecutive lanes that hold one 16-byte vector
-// each (G = 16 for 16-bit types, 32 for f32); its maximum is a shuffle
-// reduction over them. Where rows or pointers are not 16-byte aligned a warp
-// takes a block with single-element accesses, lane l elements l, l + 32, ...
+// of 128 values belongs to G consecutive lanes that hold one 32-byte vector
+// each (G = 8 for 16-bit types, 16 for f32); its maximum is a shuffle
+// reduction over them. 16-byte vectors where rows or pointers are aligned to
+// no more (half the bytes in flight: bf16 8192 x 4096 took 25.1 us, not
+// 17.9); a warp per block with single-element accesses where to less, lane l
+// elements l, l + 32, ...
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
@@ -46,12 +48,14 @@ struct RowParams {
 // instead of memory.
 __device__ __forceinline__ float silu_mul_f(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
-template <typename T, bool SILU, bool VEC>
+// W: bytes per lane and operand, 32 or 16, or 0 for single elements.
+template <typename T, bool SILU, int W>
 __global__ void __launch_bounds__(kRowThreads) rows_f8_kernel(const RowParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
-    constexpr int N = VEC ? Vec<T>::N : 4;
+    constexpr int N = W ? W / (int)sizeof(T) : 4;
     constexpr int G = F8B / N;
+    constexpr int V = Vec<T>::N;
     const int lane = threadIdx.x % G;
     const int64_t gid = (int64_t)blockIdx.x * (kRowThreads / G) + threadIdx.x / G;
     const bool live = gid < p.total;
@@ -71,20 +75,39 @@ __global__ void __launch_bounds__(kRowThreads) rows_f8_kernel(const RowParams p)
     const uint8_t *yr = SILU ? p.y + row * p.y_nb1 : nullptr;
     float f[N];
     uint32_t top = 0;
-    if constexpr (VEC) {
+    if constexpr (W != 0) {
         const int64_t k = k0 + lane * N;  // k % N == 0 here: a vector lies inside the row or outside
-        const bool in = live && k < p.k;
-        uint4 v = make_uint4(0, 0, 0, 0), w = v;
-        if (in) {
-            v = ld_stream16(xr + k * sizeof(T));
-            if constexpr (SILU) w = ld_stream16(yr + k * sizeof(T));
-        }
-        Vec<T>::get(v, f);
-        if constexpr (SILU) {
-            float u[N];
-            Vec<T>::get(w, u);
+        if (live && k < p.k) {
+            uint4 v[N / V], u[N / V];
+            if constexpr (W == 32) {
+                const Wide32 a = ld_stream32(xr + k * sizeof(T));
+                v[0] = a.lo;
+                v[N / V - 1] = a.hi;
+                if constexpr (SILU) {
+                    const Wide32 c = ld_stream32(yr + k * sizeof(T));
+                    u[0] = c.lo;
+                    u[N / V - 1] = c.hi;
+                }
+            } else {
+                v[0] = ld_stream16(xr + k * sizeof(T));
+                if constexpr (SILU) u[0] = ld_stream16(yr + k * sizeof(T));
+            }
 #pragma unroll
-            for (int i = 0; i < N; i++) f[i] = silu_mul_f(f[i], u[i]);
+            for (int h = 0; h < N / V; h++) {
+                float x[V];
+                Vec<T>::get(v[h], x);
+                if constexpr (SILU) {
+                    float y[V];
+                    Vec<T>::get(u[h], y);
+#pragma unroll
+                    for (int i = 0; i < V; i++) x[i] = silu_mul_f(x[i], y[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < V; i++) f[h * V + i] = x[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) f[i] = 0.0f;
         }
     } else {
 #pragma unroll
@@ -105,16 +128,18 @@ __global__ void __launch_bounds__(kRowThreads) rows_f8_kernel(const RowParams p)
     f8_scale(top, s, r);
     if (!live) return;
     uint8_t *qr = p.q + row * p.q_nb1;
-    if constexpr (VEC) {
+    if constexpr (W != 0) {
         const int64_t k = k0 + lane * N;
         if (k < p.k) {
-            const uint32_t lo = f8_pack4(f[0] * r, f[1] * r, f[2] * r, f[3] * r);
-            if constexpr (N == 8) {
-                const uint32_t hi = f8_pack4(f[4] * r, f[5] * r, f[6] * r, f[7] * r);
-                *reinterpret_cast<uint2 *>(qr + k) = make_uint2(lo, hi);
-            } else {
-                *reinterpret_cast<uint32_t *>(qr + k) = lo;
-            }
+            uint32_t w[N / 4];
+#pragma unroll
+            for (int i = 0; i < N / 4; i++) w[i] = f8_pack4(f[4 * i] * r, f[4 * i + 1] * r, f[4 * i + 2] * r, f[4 * i + 3] * r);
+            if constexpr (N == 16)
+                *reinterpret_cast<uint4 *>(qr + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            else if constexpr (N == 8)
+                *reinterpret_cast<uint2 *>(qr + k) = make_uint2(w[0], w[1]);
+            else
+                *reinterpret_cast<uint32_t *>(qr + k) = w[0];
         }
     } else {
 #pragma unroll
@@ -387,12 +412,12 @@ __global__ void __launch_bounds__(1024) norm_f8_any_kernel(const NormF8Params p)
 bool aligned(uint64_t a, const void *p, uint64_t nb1) { return ((reinterpret_cast<uintptr_t>(p) | nb1) & (a - 1)) == 0; }
 
 template <typename T, bool SILU>
-int launch_rows_t(const RowParams &p, bool vec, cudaStream_t s, const char *what) {
-    const int groups = kRowThreads / (vec ? F8B / Vec<T>::N : 32);
+int launch_rows_t(const RowParams &p, int width, cudaStream_t s, const char *what) {
+    const int groups = kRowThreads / (width ? F8B / (width / (int)sizeof(T)) : 32);
     const int64_t grid = (p.total + groups - 1) / groups;
     if (grid > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "%s: too many blocks", what);
-    return launch_early(what, vec ? rows_f8_kernel<T, SILU, true> : rows_f8_kernel<T, SILU, false>, dim3((unsigned)grid),
-                        dim3(kRowThreads), 0, 1, s, p);
+    auto *fn = width == 32 ? rows_f8_kernel<T, SILU, 32> : width == 16 ? rows_f8_kernel<T, SILU, 16> : rows_f8_kernel<T, SILU, 0>;
+    return launch_early(what, fn, dim3((unsigned)grid), dim3(kRowThreads), 0, 1, s, p);
 }
 
 template <typename T>
@@ -446,8 +471,11 @@ int launch_rows_f8(int32_t type, const void *x, uint64_t x_nb1, const void *up, 
     p.total = rows * p.kb;
     while ((1ull << p.kb_shift) < p.kb) p.kb_shift++;
     p.kb_mul = (uint32_t)(((1ull << 32) * ((1ull << p.kb_shift) - p.kb)) / p.kb + 1);
-    const int n = 16 / esize(type);
-    const bool vec = k % n == 0 && aligned(16, x, x_nb1) && (!up || aligned(16, up, up_nb1)) && aligned(n, o.q, o.q_nb1);
+    auto fits = [&](int w) {
+        const int n = w / esize(type);
+        return k % n == 0 && aligned(w, x, x_nb1) && (!up || aligned(w, up, up_nb1)) && aligned(n, o.q, o.q_nb1);
+    };
+    const int vec = fits(32) ? 32 : fits(16) ? 16 : 0;
     switch (type) {
         case FB_F32:
             return up ? launch_rows_t<float, true>(p, vec, s, what) : launch_rows_t<float, false>(p, vec, s, what);
