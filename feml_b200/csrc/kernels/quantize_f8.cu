@@ -262,11 +262,28 @@ __device__ __forceinline__ float cta_sum(float v, float *part) {
     return warp_sum(lane < nw ? part[lane] : 0.0f);
 }
 
-// The row in registers: NV vectors per thread. WARP: a warp per row
-// (blockDim.y rows per CTA), else a CTA per row.
-template <typename T, int NV, bool WARP>
+// W bytes (16 or 32) of a row as 16-byte vectors, and back.
+template <int W>
+__device__ __forceinline__ void ld_wide(uint4 (&v)[W / 16], const void *p) {
+    if constexpr (W == 32) {
+        const Wide32 a = ld_stream32(p);
+        v[0] = a.lo;
+        v[1] = a.hi;
+    } else {
+        v[0] = ld_stream16(p);
+    }
+}
+template <int W>
+__device__ __forceinline__ void st_wide(void *p, const uint4 (&v)[W / 16]) {
+#pragma unroll
+    for (int i = 0; i < W / 16; i++) reinterpret_cast<uint4 *>(p)[i] = v[i];
+}
+
+// The row in registers: NV vectors of W bytes per thread. WARP: a warp per
+// row (blockDim.y rows per CTA), else a CTA per row.
+template <typename T, int NV, bool WARP, int W>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8Params p) {
-    constexpr int N = Vec<T>::N, G = F8B / N;
+    constexpr int V = Vec<T>::N, H = W / 16, N = V * H, G = F8B / N;
     __shared__ float part[32];
     grid_dependency_wait();
     grid_launch_dependents();
@@ -274,41 +291,50 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8
     if (WARP && row >= p.rows) return;
     const int t = threadIdx.x, nt = WARP ? 32 : blockDim.x;
     const uint8_t *xr = p.x + row * p.x_nb1;
-    uint4 v[NV];
+    uint4 v[NV][H];
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int64_t k = (int64_t)(i * nt + t) * N;
-        v[i] = k < p.k ? ld_stream16(xr + k * sizeof(T)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int h = 0; h < H; h++) v[i][h] = make_uint4(0, 0, 0, 0);
+        if (k < p.k) ld_wide<W>(v[i], xr + k * sizeof(T));
     }
     if (p.res) {
         const uint8_t *rr = p.res + row * p.res_nb1;
         uint8_t *hr = p.sum + row * p.sum_nb1;
-        uint4 u[NV];
+        uint4 u[NV][H];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int64_t k = (int64_t)(i * nt + t) * N;
-            u[i] = k < p.k ? ld_stream16(rr + k * sizeof(T)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int h = 0; h < H; h++) u[i][h] = make_uint4(0, 0, 0, 0);
+            if (k < p.k) ld_wide<W>(u[i], rr + k * sizeof(T));
         }
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int64_t k = (int64_t)(i * nt + t) * N;
-            float a[N], b[N];
-            Vec<T>::get(v[i], a);
-            Vec<T>::get(u[i], b);
 #pragma unroll
-            for (int j = 0; j < N; j++) a[j] += b[j];
-            v[i] = Vec<T>::put(a);
-            if (k < p.k) *reinterpret_cast<uint4 *>(hr + k * sizeof(T)) = v[i];
+            for (int h = 0; h < H; h++) {
+                float a[V], b[V];
+                Vec<T>::get(v[i][h], a);
+                Vec<T>::get(u[i][h], b);
+#pragma unroll
+                for (int j = 0; j < V; j++) a[j] += b[j];
+                v[i][h] = Vec<T>::put(a);
+            }
+            if (k < p.k) st_wide<W>(hr + k * sizeof(T), v[i]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        float f[N];
-        Vec<T>::get(v[i], f);
+    for (int i = 0; i < NV; i++)
 #pragma unroll
-        for (int j = 0; j < N; j++) ss = fmaf(f[j], f[j], ss);
-    }
+        for (int h = 0; h < H; h++) {
+            float f[V];
+            Vec<T>::get(v[i][h], f);
+#pragma unroll
+            for (int j = 0; j < V; j++) ss = fmaf(f[j], f[j], ss);
+        }
     ss = WARP ? warp_sum(ss) : cta_sum(ss, part);
     const float inv = 1.0f / sqrtf(ss / (float)p.k + p.eps);
     uint8_t *qr = p.q + row * p.q_nb1;
@@ -318,40 +344,48 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8
         const int64_t k = (int64_t)(i * nt + t) * N;
         const bool in = k < p.k;
         float f[N];
-        Vec<T>::get(v[i], f);
         uint32_t top = 0;
-        if (in) {
-            float g[N];
-            if (sizeof(T) == 4 || !p.w_f32) {
-                Vec<T>::get(__ldg(reinterpret_cast<const uint4 *>(p.w + k * sizeof(T))), g);
-            } else {
 #pragma unroll
-                for (int j = 0; j < N; j += 4) {
-                    const float4 w4 = __ldg(reinterpret_cast<const float4 *>(p.w + (k + j) * 4));
-                    g[j] = w4.x;
-                    g[j + 1] = w4.y;
-                    g[j + 2] = w4.z;
-                    g[j + 3] = w4.w;
+        for (int h = 0; h < H; h++) {
+            float x[V];
+            Vec<T>::get(v[i][h], x);
+            if (in) {
+                float g[V];
+                if (sizeof(T) == 4 || !p.w_f32) {
+                    Vec<T>::get(__ldg(reinterpret_cast<const uint4 *>(p.w + (k + h * V) * sizeof(T))), g);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) {
+                        const float4 w4 = __ldg(reinterpret_cast<const float4 *>(p.w + (k + h * V + j) * 4));
+                        g[j] = w4.x;
+                        g[j + 1] = w4.y;
+                        g[j + 2] = w4.z;
+                        g[j + 3] = w4.w;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    x[j] = x[j] * inv * g[j];
+                    top = max(top, abs_bits(x[j]));
                 }
             }
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                f[j] = f[j] * inv * g[j];
-                top = max(top, abs_bits(f[j]));
-            }
+            for (int j = 0; j < V; j++) f[h * V + j] = x[j];
         }
 #pragma unroll
         for (int o = 1; o < G; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         float s, r;
         f8_scale(top, s, r);
         if (in) {
-            const uint32_t lo = f8_pack4(f[0] * r, f[1] * r, f[2] * r, f[3] * r);
-            if constexpr (N == 8) {
-                const uint32_t hi = f8_pack4(f[4] * r, f[5] * r, f[6] * r, f[7] * r);
-                *reinterpret_cast<uint2 *>(qr + k) = make_uint2(lo, hi);
-            } else {
-                *reinterpret_cast<uint32_t *>(qr + k) = lo;
-            }
+            uint32_t w[N / 4];
+#pragma unroll
+            for (int j = 0; j < N / 4; j++) w[j] = f8_pack4(f[4 * j] * r, f[4 * j + 1] * r, f[4 * j + 2] * r, f[4 * j + 3] * r);
+            if constexpr (N == 16)
+                *reinterpret_cast<uint4 *>(qr + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            else if constexpr (N == 8)
+                *reinterpret_cast<uint2 *>(qr + k) = make_uint2(w[0], w[1]);
+            else
+                *reinterpret_cast<uint32_t *>(qr + k) = w[0];
             if (t % G == 0) sr[k / F8B] = s;
         }
     }
@@ -359,6 +393,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8
 
 // Rows of any length and alignment: the sum of squares in one pass, the norm
 // in a second one that reads the stored sum (or x) again, a warp per block.
+// (A variant that held such rows in registers took 1.6 times as long at 4001 x
+// 4101 bf16: single elements need the occupancy more than the saved pass.)
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_f8_any_kernel(const NormF8Params p) {
     __shared__ float part[32];
@@ -420,34 +456,33 @@ int launch_rows_t(const RowParams &p, int width, cudaStream_t s, const char *wha
     return launch_early(what, fn, dim3((unsigned)grid), dim3(kRowThreads), 0, 1, s, p);
 }
 
-template <typename T>
-int launch_norm_t(const NormF8Params &p, bool vec, cudaStream_t s) {
+template <typename T, int W>
+int launch_norm_w(const NormF8Params &p, cudaStream_t s) {
     const char *what = "rms_norm_f8";
-    constexpr int N = Vec<T>::N;
-    const int64_t vecs = p.k / N;
-    if (!vec || vecs > 8 * 1024) {
-        const int threads = (int)std::min<int64_t>(1024, (p.k + 31) / 32 * 32);
-        return launch_early(what, norm_f8_any_kernel<T>, dim3((unsigned)p.rows), dim3(threads), 0, 1, s, p);
-    }
+    const int64_t vecs = p.k / (W / (int)sizeof(T));
     // A warp per row for short rows in numbers that fill the GPU; else a CTA
     // per row: one vector per thread when rows are few (latency), more
-    // vectors and small CTAs when they are many.
-    if (vecs <= 128 && p.rows >= 1024) {
-        const dim3 block(32, 8);
-        const unsigned grid = (unsigned)((p.rows + 7) / 8);
-        auto *fn = vecs <= 32 ? norm_f8_kernel<T, 1, true> : vecs <= 64 ? norm_f8_kernel<T, 2, true> : norm_f8_kernel<T, 4, true>;
-        return launch_early(what, fn, dim3(grid), block, 0, 1, s, p);
+    // vectors and smaller CTAs when they are many (2048 rows of 16384 f16:
+    // 41.4 us with 512 threads, 47.6 with 256, 49.7 with 1024).
+    if (vecs <= 64 && p.rows >= 1024) {
+        auto *fn = vecs <= 32 ? norm_f8_kernel<T, 1, true, W> : norm_f8_kernel<T, 2, true, W>;
+        return launch_early(what, fn, dim3((unsigned)((p.rows + 7) / 8)), dim3(32, 8), 0, 1, s, p);
     }
-    const int most = p.rows <= 296 ? 1024 : 256;
+    const int most = p.rows <= 296 ? 1024 : 512;
     int nv = 1;
-    while (nv < 8 && (vecs + nv - 1) / nv > most) nv *= 2;
+    while (nv < 4 && (vecs + nv - 1) / nv > most) nv *= 2;
     const int threads = (int)(((vecs + nv - 1) / nv + 31) / 32 * 32);
-    const unsigned grid = (unsigned)p.rows;
-    auto *fn = nv == 1   ? norm_f8_kernel<T, 1, false>
-               : nv == 2 ? norm_f8_kernel<T, 2, false>
-               : nv == 4 ? norm_f8_kernel<T, 4, false>
-                         : norm_f8_kernel<T, 8, false>;
-    return launch_early(what, fn, dim3(grid), dim3(threads), 0, 1, s, p);
+    auto *fn = nv == 1 ? norm_f8_kernel<T, 1, false, W> : nv == 2 ? norm_f8_kernel<T, 2, false, W> : norm_f8_kernel<T, 4, false, W>;
+    return launch_early(what, fn, dim3((unsigned)p.rows), dim3(threads), 0, 1, s, p);
+}
+
+// `width`: bytes that rows and pointers are aligned to, 32, 16 or 0.
+template <typename T>
+int launch_norm_t(const NormF8Params &p, int width, cudaStream_t s) {
+    if (width == 32 && p.k * (int64_t)sizeof(T) <= 32 * 4 * 1024) return launch_norm_w<T, 32>(p, s);
+    if (width && p.k * (int64_t)sizeof(T) <= 16 * 4 * 1024) return launch_norm_w<T, 16>(p, s);
+    const int threads = (int)std::min<int64_t>(1024, (p.k + 31) / 32 * 32);
+    return launch_early("rms_norm_f8", norm_f8_any_kernel<T>, dim3((unsigned)p.rows), dim3(threads), 0, 1, s, p);
 }
 
 int esize(int32_t type) { return type == FB_F32 ? 4 : 2; }
@@ -528,10 +563,12 @@ int launch_rms_norm_f8(int32_t type, const void *x, uint64_t x_nb1, const void *
     p.rows = rows;
     p.k = k;
     p.eps = eps;
-    const int n = 16 / esize(type);
-    const bool vec = k % n == 0 && aligned(16, x, x_nb1) && aligned(16, weight, 0) &&
-                     (!residual || (aligned(16, residual, residual_nb1) && aligned(16, sum, sum_nb1))) &&
-                     aligned(n, o.q, o.q_nb1);
+    auto fits = [&](int w) {
+        const int n = w / esize(type);
+        return k % n == 0 && aligned(w, x, x_nb1) && aligned(16, weight, 0) &&
+               (!residual || (aligned(w, residual, residual_nb1) && aligned(16, sum, sum_nb1))) && aligned(n, o.q, o.q_nb1);
+    };
+    const int vec = fits(32) ? 32 : fits(16) ? 16 : 0;
     switch (type) {
         case FB_F32: return launch_norm_t<float>(p, vec, s);
         case FB_F16: return launch_norm_t<__half>(p, vec, s);
