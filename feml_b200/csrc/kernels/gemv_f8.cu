@@ -2,18 +2,19 @@
 // once, straight into tensor-core fragments.
 //
 // A warp takes 32 weight rows x one block of 128 values at a time: thread
-// (g, t) of the m16n8k16 layout loads the 16-byte units t and t + 4 of rows
-// g, g + 8, g + 16 and g + 24. The layout's own order of k within a row does
-// not matter to a sum as long as both operands use the same one, so a 32-bit
-// word of each row serves one MMA and nothing is shuffled. The words are
-// widened to f16 on the way (exact; the sum is f32): the MMA that takes e4m3
-// itself measured about 100 cycles per instruction here, several times the
-// conversions and f16 MMAs that replace it. The products of a block are
-// scaled in registers; the eight warps of a CTA take blocks in turn and meet
-// in shared memory in warp order. Few weight rows: a cluster of S CTAs splits
-// the blocks further and adds its partial sums in rank order through
-// distributed shared memory. Bound by memory: each warp has two blocks (8 KB
-// of weights) in flight.
+// (g, t) of the m16n8k16 layout loads bytes 32 t to 32 t + 31 of rows g, g + 8,
+// g + 16 and g + 24. The layout's own order of k within a row does not matter
+// to a sum as long as both operands use the same one, so a 32-bit word of each
+// row serves one MMA and nothing is shuffled. The words are widened to f16 on
+// the way (exact; the sum is f32): the MMA that takes e4m3 itself measured
+// about 100 cycles per instruction here, several times the conversions and
+// f16 MMAs that replace it. The products of a block are scaled in registers;
+// the warps of a CTA take blocks in turn and meet in shared memory in warp
+// order. Few weight rows: a cluster of S CTAs splits the blocks further and
+// adds its partial sums in rank order through distributed shared memory.
+// Bound by memory: each warp has two blocks (8 KB of weights) in flight (one
+// row, 4096 x 4096: 5.0 us, 3.3 TB/s; 4096 x 14336: 13.9 us, 4.2 TB/s; launch
+// and one memory round trip are 3 us of either).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -25,10 +26,8 @@ namespace fbk {
 
 namespace {
 
-constexpr int V_WARPS = 8;
 constexpr int V_TILES = 2;   // m16 tiles of weight rows per warp
 constexpr int V_ROWS = 16 * V_TILES;
-constexpr int V_AHEAD = 2;   // blocks (4 KB each) in flight per warp
 
 // The 16-byte unit at `p`, of which `n` bytes exist (the end of a row).
 __device__ __forceinline__ uint4 ld_unit(const uint8_t *p, int n) {
@@ -51,9 +50,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// NT: groups of eight rows of x.
-template <int NT, typename T>
-__global__ void __launch_bounds__(32 * V_WARPS) gemv_f8_kernel(const F8Gemm p, int splits) {
+// NT: groups of eight rows of x. WIDE: weight rows aligned to 32 bytes.
+// V_WARPS: warps that take blocks in turn.
+template <int V_WARPS, int NT, bool WIDE, typename T>
+__global__ void __launch_bounds__(32 * V_WARPS, V_WARPS == 8 && NT == 1 ? 2 : 1) gemv_f8_kernel(const F8Gemm p, int splits) {
     __shared__ float part[V_WARPS][NT * 8][V_ROWS + 1];
     grid_dependency_wait();
     grid_launch_dependents();
@@ -62,12 +62,12 @@ __global__ void __launch_bounds__(32 * V_WARPS) gemv_f8_kernel(const F8Gemm p, i
     const int kb = (p.K + F8B - 1) / F8B;
     const uint8_t *w[2 * V_TILES];
 #pragma unroll
-    for (int i = 0; i < 2 * V_TILES; i++) w[i] = p.w + (uint64_t)min(m0 + g + 8 * i, p.M - 1) * p.w_nb1 + t * 16;
+    for (int i = 0; i < 2 * V_TILES; i++) w[i] = p.w + (uint64_t)min(m0 + g + 8 * i, p.M - 1) * p.w_nb1 + t * 32;
     const uint8_t *x[NT];
     const float *xs[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        x[n] = p.x + (uint64_t)min(n * 8 + g, p.N - 1) * p.x_nb1 + t * 16;
+        x[n] = p.x + (uint64_t)min(n * 8 + g, p.N - 1) * p.x_nb1 + t * 32;
 #pragma unroll
         for (int h = 0; h < 2; h++)
             xs[n][h] = reinterpret_cast<const float *>(p.xs + (uint64_t)min(n * 8 + 2 * t + h, p.N - 1) * p.xs_nb1);
@@ -102,50 +102,53 @@ __global__ void __launch_bounds__(32 * V_WARPS) gemv_f8_kernel(const F8Gemm p, i
                 for (int h = 0; h < 4; h++) acc[n][i][h] = fmaf(d[n][i][h], s[n][h & 1], acc[n][i][h]);
     };
     const int whole = p.K / F8B, step = V_WARPS * splits;
-    for (int b0 = rank * V_WARPS + warp; b0 < whole; b0 += step * V_AHEAD) {
-        uint4 a[V_AHEAD][2 * V_TILES][2], xv[V_AHEAD][NT][2];
-        float s[V_AHEAD][NT][2];
+    auto fetch = [&](int b, uint4 (&a)[2 * V_TILES][2]) {
 #pragma unroll
-        for (int i = 0; i < V_AHEAD; i++) {
-            const int b = b0 + i * step;
-            if (b >= whole) break;
-#pragma unroll
-            for (int r = 0; r < 2 * V_TILES; r++) {
-                a[i][r][0] = ld_stream16(w[r] + (int64_t)b * F8B);
-                a[i][r][1] = ld_stream16(w[r] + (int64_t)b * F8B + 64);
+        for (int r = 0; r < 2 * V_TILES; r++) {
+            const uint8_t *q = w[r] + (int64_t)b * F8B;
+            if constexpr (WIDE) {
+                const Wide32 v = ld_stream32(q);
+                a[r][0] = v.lo;
+                a[r][1] = v.hi;
+            } else {
+                a[r][0] = ld_stream16(q);
+                a[r][1] = ld_stream16(q + 16);
             }
         }
+    };
+    auto use = [&](int b, const uint4 (&a)[2 * V_TILES][2]) {
+        uint4 xv[NT][2];
+        float s[NT][2];
+        const float sw = ws[b];
 #pragma unroll
-        for (int i = 0; i < V_AHEAD; i++) {
-            const int b = b0 + i * step;
-            if (b >= whole) break;
-            const float sw = ws[b];
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                xv[i][n][0] = *reinterpret_cast<const uint4 *>(x[n] + (int64_t)b * F8B);
-                xv[i][n][1] = *reinterpret_cast<const uint4 *>(x[n] + (int64_t)b * F8B + 64);
-                s[i][n][0] = xs[n][0][b] * sw;
-                s[i][n][1] = xs[n][1][b] * sw;
-            }
+        for (int n = 0; n < NT; n++) {
+            xv[n][0] = *reinterpret_cast<const uint4 *>(x[n] + (int64_t)b * F8B);
+            xv[n][1] = *reinterpret_cast<const uint4 *>(x[n] + (int64_t)b * F8B + 16);
+            s[n][0] = xs[n][0][b] * sw;
+            s[n][1] = xs[n][1][b] * sw;
         }
-#pragma unroll
-        for (int i = 0; i < V_AHEAD; i++) {
-            if (b0 + i * step >= whole) break;
-            product(a[i], xv[i], s[i]);
-        }
+        product(a, xv, s);
+    };
+    int b = rank * V_WARPS + warp;
+    for (; b < whole; b += 2 * step) {
+        uint4 a0[2 * V_TILES][2], a1[2 * V_TILES][2];
+        fetch(b, a0);
+        if (b + step < whole) fetch(b + step, a1);
+        use(b, a0);
+        if (b + step < whole) use(b + step, a1);
     }
     if (whole < kb && whole % step == rank * V_WARPS + warp) {  // the row's last, shorter block
         uint4 a[2 * V_TILES][2], xv[NT][2];
         float s[NT][2];
-        const int k = whole * F8B, left = p.K - k - t * 16;
+        const int k = whole * F8B, left = p.K - k - t * 32;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int n1 = left - 64 * h;
+            const int n1 = left - 16 * h;
 #pragma unroll
-            for (int r = 0; r < 2 * V_TILES; r++) a[r][h] = ld_unit(w[r] + k + 64 * h, n1);
+            for (int r = 0; r < 2 * V_TILES; r++) a[r][h] = ld_unit(w[r] + k + 16 * h, n1);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                xv[n][h] = ld_unit(x[n] + k + 64 * h, n1);
+                xv[n][h] = ld_unit(x[n] + k + 16 * h, n1);
                 s[n][h] = xs[n][h][whole] * ws[whole];
             }
         }
@@ -187,9 +190,21 @@ __global__ void __launch_bounds__(32 * V_WARPS) gemv_f8_kernel(const F8Gemm p, i
     }
 }
 
-template <int NT, typename T>
+template <int V_WARPS, int NT, bool WIDE, typename T>
 int launch_v(const F8Gemm &p, int ctas, int splits, cudaStream_t s) {
-    return launch_early("mul_mat_f8", gemv_f8_kernel<NT, T>, dim3((unsigned)ctas), dim3(32 * V_WARPS), 0, splits, s, p, splits);
+    return launch_early("mul_mat_f8", gemv_f8_kernel<V_WARPS, NT, WIDE, T>, dim3((unsigned)ctas), dim3(32 * V_WARPS), 0, splits, s, p, splits);
+}
+
+template <int V_WARPS, typename T>
+int launch_n(const F8Gemm &p, int ctas, int splits, cudaStream_t s) {
+    const bool wide = ((reinterpret_cast<uintptr_t>(p.w) | p.w_nb1) & 31) == 0;
+    if (p.N <= 8) return wide ? launch_v<V_WARPS, 1, true, T>(p, ctas, splits, s) : launch_v<V_WARPS, 1, false, T>(p, ctas, splits, s);
+    return wide ? launch_v<V_WARPS, 2, true, T>(p, ctas, splits, s) : launch_v<V_WARPS, 2, false, T>(p, ctas, splits, s);
+}
+
+template <typename T>
+int launch_w(const F8Gemm &p, int warps, int ctas, int splits, cudaStream_t s) {
+    return warps == 16 ? launch_n<16, T>(p, ctas, splits, s) : launch_n<8, T>(p, ctas, splits, s);
 }
 
 }  // namespace
@@ -199,15 +214,20 @@ int gemv_f8_max_rows() { return 16; }
 int launch_gemv_f8(const F8Gemm &p, cudaStream_t s) {
     const int64_t tiles = ((int64_t)p.M + V_ROWS - 1) / V_ROWS;
     const int kb = (p.K + F8B - 1) / F8B;
-    // split the blocks until two CTAs per SM are busy, eight warps with a block each
+    // Two CTAs of eight warps per SM where there are tiles enough; one of
+    // sixteen where there are not (one row, 4096 x 4096: 5.0 us, with eight
+    // warps 6.7, with clusters of two 8.7); clusters of eight-warp CTAs only
+    // where the tiles do not reach half of the SMs (16384 x 512: 5.4 us with
+    // eight CTAs per tile, 17 with one).
+    const bool few = tiles * 2 <= sm_count();
+    const int warps = few || tiles >= 2 * sm_count() || kb < 16 ? 8 : 16;
     int splits = 1;
-    while (splits < 8 && tiles * splits < 2 * sm_count() && kb >= 2 * splits * V_WARPS) splits *= 2;
+    while (few && splits < 8 && tiles * splits * 2 <= sm_count() && kb >= 2 * splits * warps) splits *= 2;
     if (tiles * splits > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: too many tiles");
     const int ctas = (int)(tiles * splits);
-    const bool one = p.N <= 8;
-    if (p.out_type == FB_F32) return one ? launch_v<1, float>(p, ctas, splits, s) : launch_v<2, float>(p, ctas, splits, s);
-    if (p.out_type == FB_F16) return one ? launch_v<1, __half>(p, ctas, splits, s) : launch_v<2, __half>(p, ctas, splits, s);
-    return one ? launch_v<1, __nv_bfloat16>(p, ctas, splits, s) : launch_v<2, __nv_bfloat16>(p, ctas, splits, s);
+    if (p.out_type == FB_F32) return launch_w<float>(p, warps, ctas, splits, s);
+    if (p.out_type == FB_F16) return launch_w<__half>(p, warps, ctas, splits, s);
+    return launch_w<__nv_bfloat16>(p, warps, ctas, splits, s);
 }
 
 }  // namespace fbk
