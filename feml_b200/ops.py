@@ -236,38 +236,44 @@ def _f8_refuse(op, name, t, dtype, shape, device):
 
 def _f8_check(op, name, t, dtype, shape, device):
     """The tensor of an operand: on CUDA device `device`, of `dtype` and
-    `shape`, its last dimension contiguous."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device
-            and (t.stride(-1) == 1 or shape[-1] <= 1)):
-        _f8_refuse(op, name, t, dtype, shape, device)
+    `shape`, its last dimension contiguous. Returns its strides."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device:
+        strides = t.stride()
+        if not strides or strides[-1] == 1 or shape[-1] <= 1:
+            return strides
+    _f8_refuse(op, name, t, dtype, shape, device)
 
 
 def _f8_input(op, name, x):
-    """Type id of a 2D activation matrix."""
+    """(type id, rows, k, row stride in bytes) of a 2D activation matrix."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise FemlError("msg", f"{op}: {name} is not a CUDA tensor")
-    if x.dim() != 2:
-        raise FemlError("shape", f"{op}: {name} is {list(x.shape)}, not 2-dimensional")
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 2:
+        raise FemlError("shape", f"{op}: {name} is {list(shape)}, not 2-dimensional")
     tid = _F8_TYPES.get(x.dtype)
     if tid is None:
         raise FemlError("unsupported", f"{op}: {name} is {x.dtype} (float32, float16 and bfloat16)")
-    if x.stride(1) != 1 and x.shape[1] > 1:
+    if strides[1] != 1 and shape[1] > 1:
         raise FemlError("shape", f"{op}: the rows of {name} are not contiguous")
-    return tid
+    return tid, shape[0], shape[1], strides[0] * (4 if tid == 5 else 2)
 
 
 def _f8_out(op, out, scale, rows, k, block_rows, device):
-    """The two outputs of a quantizing call, given or new."""
+    """The two outputs of a quantizing call, given or new, and the arguments
+    that stand for them."""
     srows, kb = -(-rows // block_rows), -(-k // 128)
     if out is None:
         out = torch.empty((rows, k), dtype=_F8, device=f"cuda:{device}")
+        nb1 = k
     else:
-        _f8_check(op, "out", out, _F8, (rows, k), device)
+        nb1 = _f8_check(op, "out", out, _F8, (rows, k), device)[0]
     if scale is None:
         scale = torch.empty((srows, kb), dtype=_F32, device=f"cuda:{device}")
+        scale_nb1 = kb * 4
     else:
-        _f8_check(op, "scale", scale, _F32, (srows, kb), device)
-    return out, scale
+        scale_nb1 = _f8_check(op, "scale", scale, _F32, (srows, kb), device)[0] * 4
+    return out, scale, (out.data_ptr(), nb1, scale.data_ptr(), scale_nb1)
 
 
 def _f8_call(device, fn, *args):
@@ -286,13 +292,12 @@ def quantize_f8(x, block_rows=1, out=None, scale=None):
     scale f32 [ceil(rows / block_rows), ceil(k / 128)]): block_rows = 1 for
     activations, 128 for weights."""
     op = "quantize_f8"
-    tid = _f8_input(op, "x", x)
+    tid, rows, k, nb1 = _f8_input(op, "x", x)
     if block_rows not in (1, 128):
         raise FemlError("unsupported", f"{op}: blocks of {block_rows} rows (1 or 128)")
-    rows, k = x.shape
-    out, scale = _f8_out(op, out, scale, rows, k, block_rows, x.get_device())
-    _f8_call(x.get_device(), _L.lib().feml_b200_quantize_f8, tid, x.data_ptr(), x.stride(0) * x.element_size(), rows, k,
-             block_rows, out.data_ptr(), out.stride(0), scale.data_ptr(), scale.stride(0) * 4)
+    dev = x.get_device()
+    out, scale, o = _f8_out(op, out, scale, rows, k, block_rows, dev)
+    _f8_call(dev, _L.lib().feml_b200_quantize_f8, tid, x.data_ptr(), nb1, rows, k, block_rows, *o)
     return out, scale
 
 
@@ -302,29 +307,25 @@ def rms_norm_f8(x, weight, eps, residual=None, residual_out=None, out=None, scal
     x, residual [rows, k]; weight [k] of x's type or f32. h is written to
     `residual_out`, which may be x or residual itself."""
     op = "rms_norm_f8"
-    tid = _f8_input(op, "x", x)
-    rows, k = x.shape
-    dev, es = x.get_device(), x.element_size()
-    if isinstance(weight, torch.Tensor) and weight.dtype == torch.float32:
-        wid = 5
-        _f8_check(op, "weight", weight, torch.float32, (k,), dev)
-    else:
-        wid = tid
-        _f8_check(op, "weight", weight, x.dtype, (k,), dev)
+    tid, rows, k, nb1 = _f8_input(op, "x", x)
+    dev = x.get_device()
+    wid = 5 if isinstance(weight, torch.Tensor) and weight.dtype is _F32 else tid
+    _f8_check(op, "weight", weight, _F32 if wid == 5 else x.dtype, (k,), dev)
     r_ptr = r_nb1 = h_ptr = h_nb1 = 0
     if residual is not None:
-        _f8_check(op, "residual", residual, x.dtype, (rows, k), dev)
+        es = 4 if tid == 5 else 2
+        r_nb1 = _f8_check(op, "residual", residual, x.dtype, (rows, k), dev)[0] * es
         if residual_out is None:
             residual_out = torch.empty((rows, k), dtype=x.dtype, device=x.device)
+            h_nb1 = k * es
         else:
-            _f8_check(op, "residual_out", residual_out, x.dtype, (rows, k), dev)
-        r_ptr, r_nb1 = residual.data_ptr(), residual.stride(0) * es
-        h_ptr, h_nb1 = residual_out.data_ptr(), residual_out.stride(0) * es
+            h_nb1 = _f8_check(op, "residual_out", residual_out, x.dtype, (rows, k), dev)[0] * es
+        r_ptr, h_ptr = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise FemlError("msg", f"{op}: residual_out without a residual")
-    out, scale = _f8_out(op, out, scale, rows, k, 1, dev)
-    _f8_call(dev, _L.lib().feml_b200_rms_norm_f8, tid, x.data_ptr(), x.stride(0) * es, r_ptr, r_nb1, h_ptr, h_nb1, wid,
-             weight.data_ptr(), eps, rows, k, out.data_ptr(), out.stride(0), scale.data_ptr(), scale.stride(0) * 4)
+    out, scale, o = _f8_out(op, out, scale, rows, k, 1, dev)
+    _f8_call(dev, _L.lib().feml_b200_rms_norm_f8, tid, x.data_ptr(), nb1, r_ptr, r_nb1, h_ptr, h_nb1, wid,
+             weight.data_ptr(), eps, rows, k, *o)
     return out, scale, residual_out
 
 
@@ -332,27 +333,23 @@ def silu_mul_f8(gate, up, out=None, scale=None):
     """gate / (1 + exp(-gate)) * up in the 8-bit form -> (q, scale). gate and
     up [rows, k], for instance the two halves of one product's output."""
     op = "silu_mul_f8"
-    tid = _f8_input(op, "gate", gate)
-    rows, k = gate.shape
+    tid, rows, k, nb1 = _f8_input(op, "gate", gate)
     dev = gate.get_device()
-    _f8_check(op, "up", up, gate.dtype, (rows, k), dev)
-    out, scale = _f8_out(op, out, scale, rows, k, 1, dev)
-    es = gate.element_size()
-    _f8_call(dev, _L.lib().feml_b200_silu_mul_f8, tid, gate.data_ptr(), gate.stride(0) * es, up.data_ptr(),
-             up.stride(0) * es, rows, k, out.data_ptr(), out.stride(0), scale.data_ptr(), scale.stride(0) * 4)
+    up_nb1 = _f8_check(op, "up", up, gate.dtype, (rows, k), dev)[0] * (4 if tid == 5 else 2)
+    out, scale, o = _f8_out(op, out, scale, rows, k, 1, dev)
+    _f8_call(dev, _L.lib().feml_b200_silu_mul_f8, tid, gate.data_ptr(), nb1, up.data_ptr(), up_nb1, rows, k, *o)
     return out, scale
 
 
 def _f8_dst(op, out, out_dtype, n, m, device):
-    """Output of a product and its type id; f32 unless given."""
+    """Output of a product (f32 unless given), its type id and row stride in bytes."""
     if out is None:
         out = torch.empty((n, m), dtype=out_dtype or _F32, device=f"cuda:{device}")
-    else:
-        _f8_check(op, "out", out, out_dtype or out.dtype, (n, m), device)
+    nb1 = _f8_check(op, "out", out, out_dtype or getattr(out, "dtype", None), (n, m), device)[0]
     tid = _F8_TYPES.get(out.dtype)
     if tid is None:
         raise FemlError("unsupported", f"{op}: out is {out.dtype} (float32, float16 and bfloat16)")
-    return out, tid
+    return out, tid, nb1 * (4 if tid == 5 else 2)
 
 
 def mul_mat_f8(w, w_scale, x, x_scale, out=None, out_dtype=None):
@@ -367,14 +364,13 @@ def mul_mat_f8(w, w_scale, x, x_scale, out=None, out_dtype=None):
     dev = w.get_device()
     m, k = w.shape
     n, kb = x.shape[0], -(-k // 128)
-    _f8_check(op, "w", w, _F8, (m, k), dev)
-    _f8_check(op, "w_scale", w_scale, torch.float32, (-(-m // 128), kb), dev)
-    _f8_check(op, "x", x, _F8, (n, k), dev)
-    _f8_check(op, "x_scale", x_scale, torch.float32, (n, kb), dev)
-    out, tid = _f8_dst(op, out, out_dtype, n, m, dev)
-    _f8_call(dev, _L.lib().feml_b200_mul_mat_f8, w.data_ptr(), w.stride(0), w_scale.data_ptr(), w_scale.stride(0) * 4,
-             x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0) * 4, tid, out.data_ptr(),
-             out.stride(0) * out.element_size(), k, m, n)
+    w_nb1 = _f8_check(op, "w", w, _F8, (m, k), dev)[0]
+    ws_nb1 = _f8_check(op, "w_scale", w_scale, _F32, (-(-m // 128), kb), dev)[0] * 4
+    x_nb1 = _f8_check(op, "x", x, _F8, (n, k), dev)[0]
+    xs_nb1 = _f8_check(op, "x_scale", x_scale, _F32, (n, kb), dev)[0] * 4
+    out, tid, nb1 = _f8_dst(op, out, out_dtype, n, m, dev)
+    _f8_call(dev, _L.lib().feml_b200_mul_mat_f8, w.data_ptr(), w_nb1, w_scale.data_ptr(), ws_nb1, x.data_ptr(), x_nb1,
+             x_scale.data_ptr(), xs_nb1, tid, out.data_ptr(), nb1, k, m, n)
     return out
 
 
@@ -403,10 +399,10 @@ def mul_mat_f8_grouped(w, w_scale, x, x_scale, counts, offsets, rows=None, n_sel
     dev = w.get_device()
     e, m, k = w.shape
     n, kb = x.shape[0], -(-k // 128)
-    _f8_check(op, "w", w, _F8, (e, m, k), dev)
-    _f8_check(op, "w_scale", w_scale, torch.float32, (e, -(-m // 128), kb), dev)
-    _f8_check(op, "x", x, _F8, (n, k), dev)
-    _f8_check(op, "x_scale", x_scale, torch.float32, (n, kb), dev)
+    w_nb2, w_nb1, _ = _f8_check(op, "w", w, _F8, (e, m, k), dev)
+    ws_nb2, ws_nb1, _ = _f8_check(op, "w_scale", w_scale, _F32, (e, -(-m // 128), kb), dev)
+    x_nb1 = _f8_check(op, "x", x, _F8, (n, k), dev)[0]
+    xs_nb1 = _f8_check(op, "x_scale", x_scale, _F32, (n, kb), dev)[0]
     _f8_check(op, "counts", counts, torch.int32, (e,), dev)
     _f8_check(op, "offsets", offsets, torch.int32, (e,), dev)
     n_rows = n
@@ -425,13 +421,12 @@ def mul_mat_f8_grouped(w, w_scale, x, x_scale, counts, offsets, rows=None, n_sel
         _f8_check(op, "status", status, torch.int32, (1,), dev)
     if out is None:
         out = torch.zeros((n_rows, m), dtype=out_dtype or _F32, device=w.device)
-    out, tid = _f8_dst(op, out, out_dtype, n_rows, m, dev)
-    _f8_call(dev, _L.lib().feml_b200_mul_mat_f8_grouped, w.data_ptr(), w.stride(1), w.stride(0), w_scale.data_ptr(),
-             w_scale.stride(1) * 4, w_scale.stride(0) * 4, e, x.data_ptr(), x.stride(0), n, x_scale.data_ptr(),
-             x_scale.stride(0) * 4, counts.data_ptr(), offsets.data_ptr(), rows.data_ptr() if rows is not None else 0,
-             int(n_selected), tid, out.data_ptr(), out.stride(0) * out.element_size(), k, m, n_rows,
-             workspace.data_ptr() if workspace is not None else 0, workspace.numel() if workspace is not None else 0,
-             status.data_ptr() if status is not None else 0)
+    out, tid, nb1 = _f8_dst(op, out, out_dtype, n_rows, m, dev)
+    _f8_call(dev, _L.lib().feml_b200_mul_mat_f8_grouped, w.data_ptr(), w_nb1, w_nb2, w_scale.data_ptr(), ws_nb1 * 4,
+             ws_nb2 * 4, e, x.data_ptr(), x_nb1, n, x_scale.data_ptr(), xs_nb1 * 4, counts.data_ptr(),
+             offsets.data_ptr(), rows.data_ptr() if rows is not None else 0, int(n_selected), tid, out.data_ptr(), nb1, k, m,
+             n_rows, workspace.data_ptr() if workspace is not None else 0,
+             workspace.numel() if workspace is not None else 0, status.data_ptr() if status is not None else 0)
     return out
 
 
