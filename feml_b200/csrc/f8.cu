@@ -44,7 +44,8 @@ int check_type(const char *op, int32_t type) {
 
 int check_dims(const char *op, int64_t a, int64_t b, int64_t c) {
     if (a < 0 || b < 0 || c < 0) return set_error(FB_ERR_INVALID, "%s: negative dimension", op);
-    if (a > INT32_MAX || b > INT32_MAX || c > INT32_MAX) return set_error(FB_ERR_UNSUPPORTED, "%s: dimension over 2^31", op);
+    constexpr int64_t most = INT32_MAX - 1024;  // a tile's end still fits an int
+    if (a > most || b > most || c > most) return set_error(FB_ERR_UNSUPPORTED, "%s: dimension over 2^31 - 1025", op);
     return FB_OK;
 }
 

@@ -85,6 +85,7 @@ struct GParams {
     int tiles_m, tiles_n;  // tiles of weight rows; of rows (ungrouped)
     int band;              // row tiles walked together (ungrouped)
     int kb;                // blocks
+    int max_tiles;         // grouped: the most that groups which do not overlap can need
 };
 
 struct GTile {
@@ -328,21 +329,29 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     grid_dependency_wait();
     grid_launch_dependents();
     if (warp == 3 && p.g.counts) {  // first tile of every group
+        // (overlapping groups could ask for any number of tiles: no more than
+        // max_tiles are walked)
         int run = 0;
+        bool over = false;
         for (int e0 = 0; e0 < p.g.n_experts; e0 += 32) {
             int n = 0;
             if (e0 + lane < p.g.n_experts)
                 n = (f8_group(p.g, e0 + lane, blockIdx.x == 0 ? p.status : nullptr).rows + GM - 1) / GM * q.tiles_m;
-            int sum = n;
+            int64_t sum = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += v;
             }
-            if (e0 + lane < p.g.n_experts) start[e0 + lane] = run + sum - n;
-            run += __shfl_sync(0xffffffffu, sum, 31);
+            if (e0 + lane < p.g.n_experts) start[e0 + lane] = (int)min(run + sum - n, (int64_t)q.max_tiles);
+            const int64_t all = run + __shfl_sync(0xffffffffu, sum, 31);
+            over = over || all > q.max_tiles;
+            run = (int)min(all, (int64_t)q.max_tiles);
         }
-        if (lane == 0) start[p.g.n_experts] = run;
+        if (lane == 0) {
+            start[p.g.n_experts] = run;
+            if (over && blockIdx.x == 0) report_status(p.status, STATUS_BAD_ID);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -553,7 +562,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         cluster_arrive();
         cluster_wait();
         const GTile tile = g_tile(q, start, t0, BN);
-        if (warp >= 4 && tile.expert >= 0 && !*abort_flag) {
+        int broken = 0;  // in any CTA of the cluster
+        for (int i = 0; i < S; i++) broken |= (int)dsmem_ld4(dsmem_map(const_cast<const int *>(abort_flag), (uint32_t)i));
+        if (warp >= 4 && tile.expert >= 0 && !broken) {
             // rows rank, rank + S, ... : the S partial rows added in rank order
             const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | p.y_nb1) & 15) == 0;
             for (int r = rank + (warp - 4) * S; r < tile.rows; r += G_EPI_WARPS * S) {
@@ -694,6 +705,7 @@ int launch_gemm_f8(const F8Gemm &p, cudaStream_t s) {
     const int bn = nt * m256 >= sms ? 256 : 128;
     const int64_t tiles = nt * (bn == 256 ? m256 : m128);
     q.tiles_m = (int)(bn == 256 ? m256 : m128);
+    q.max_tiles = (int)tiles;
     int split = 1;
     if (bn == 128)
         while (split < 8 && tiles * split * 2 <= sms && q.kb / (split * 2) >= 2) split *= 2;

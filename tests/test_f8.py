@@ -44,7 +44,7 @@ def grouped(w=P, w_nb1=256, w_nb2=256 * 300, ws=P, ws_nb1=8, ws_nb2=24, E=4, x=P
 
 @pytest.mark.parametrize("fn,bad,code", [
     (quantize, dict(t=11), UNSUPPORTED), (quantize, dict(t=-1), UNSUPPORTED), (quantize, dict(rows=-1), INVALID),
-    (quantize, dict(k=-1), INVALID), (quantize, dict(rows=1 << 31), UNSUPPORTED), (quantize, dict(br=2), UNSUPPORTED),
+    (quantize, dict(k=-1), INVALID), (quantize, dict(rows=1 << 31), UNSUPPORTED), (mul_mat, dict(K=2 ** 31 - 1), UNSUPPORTED), (quantize, dict(br=2), UNSUPPORTED),
     (quantize, dict(br=0), UNSUPPORTED), (quantize, dict(x=0), INVALID), (quantize, dict(q=0), INVALID),
     (quantize, dict(s=0), INVALID), (quantize, dict(x=P + 2), INVALID), (quantize, dict(x_nb1=514), INVALID),
     (quantize, dict(x_nb1=508), SHAPE), (quantize, dict(x_nb1=0), SHAPE), (quantize, dict(q_nb1=127), SHAPE),

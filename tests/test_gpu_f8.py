@@ -454,6 +454,20 @@ def test_grouped_bad_tables(k, m):
     assert torch.all(big[1:4] == 0) and torch.all(big[90:] == 5.0) and int(status) == 2
 
 
+def test_grouped_overlapping_tables_end():
+    """Groups that lie inside the output one by one but overlap: reported where they add up to more rows than there
+    are, never more work than a proper table asks for, nothing outside the output."""
+    k, m, e, n = 256, 130, 40, 300
+    w, ws, x, xs = operands(2, n, k, m, e)
+    c = torch.full((e,), n, dtype=torch.int32, device="cuda")
+    o = torch.zeros(e, dtype=torch.int32, device="cuda")
+    buf = torch.full((n + 2, m), 5.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.mul_mat_f8_grouped(w, ws, x, xs, c, o, out=buf[1:n + 1], status=status)
+    assert int(status) == 2
+    assert torch.all(buf[0] == 5.0) and torch.all(buf[n + 1] == 5.0) and torch.isfinite(buf).all()
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # as they are used
 # ---------------------------------------------------------------------------------------------------------------
