@@ -564,25 +564,38 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         const GTile tile = g_tile(q, start, t0, BN);
         int broken = 0;  // in any CTA of the cluster
         for (int i = 0; i < S; i++) broken |= (int)dsmem_ld4(dsmem_map(const_cast<const int *>(abort_flag), (uint32_t)i));
-        if (warp >= 4 && tile.expert >= 0 && !broken) {
-            // rows rank, rank + S, ... : the S partial rows added in rank order
-            const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | p.y_nb1) & 15) == 0;
-            for (int r = rank + (warp - 4) * S; r < tile.rows; r += G_EPI_WARPS * S) {
-                for (int c = lane * 8; c < BN; c += 256) {
-                    float f[8] = {};
-                    for (int i = 0; i < S; i++) {
-                        const uint32_t a = dsmem_map(gbase + (r * (BN + 4) + c) * 4, (uint32_t)i);
-                        const int4 lo = dsmem_ld16(a), hi = dsmem_ld16(a + 16);
-                        const int w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        static_assert(!SPLIT || BN == 128, "four columns per lane");
+        if (tile.expert >= 0 && !broken) {
+            // rows rank, rank + S, ...: the S partial rows, all of them on the way
+            // before the first is added (one after the other they cost 3 us),
+            // in rank order
+            const int m = tile.m0 + lane * 4;
+            const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | p.y_nb1) & (4 * sizeof(T) - 1)) == 0 && m + 4 <= p.M;
+            for (int r = rank + warp * S; r < tile.rows; r += G_THREADS / 32 * S) {
+                const uint8_t *mine = gbase + (r * (BN + 4) + lane * 4) * 4;
+                int4 v[8];
 #pragma unroll
-                        for (int j = 0; j < 8; j++) f[j] += __int_as_float(w[j]);
+                for (int i = 0; i < 8; i++)
+                    if (i < S) v[i] = dsmem_ld16(dsmem_map(mine, (uint32_t)i));
+                float f[4] = {};
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (i < S) {
+                        f[0] += __int_as_float(v[i].x);
+                        f[1] += __int_as_float(v[i].y);
+                        f[2] += __int_as_float(v[i].z);
+                        f[3] += __int_as_float(v[i].w);
                     }
-                    const int m = tile.m0 + c;
-                    uint8_t *o = p.y + (uint64_t)(tile.row0 + r) * p.y_nb1;
-                    if (m < p.M) {
-                        store16<T>(o, m, p.M, pack16<T>(f), wide);
-                        if (sizeof(T) == 4 && m + 4 < p.M) store16<T>(o, m + 4, p.M, pack16<T>(f + 8 - Vec<T>::N), wide);
-                    }
+                T *o = reinterpret_cast<T *>(p.y + (uint64_t)(tile.row0 + r) * p.y_nb1) + m;
+                if (wide) {
+                    if constexpr (sizeof(T) == 4)
+                        *reinterpret_cast<float4 *>(o) = make_float4(f[0], f[1], f[2], f[3]);
+                    else
+                        *reinterpret_cast<uint2 *>(o) = make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (m + i < p.M) o[i] = from_f32<T>(f[i]);
                 }
             }
         }
