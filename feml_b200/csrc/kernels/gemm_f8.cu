@@ -11,27 +11,31 @@
 // Roles of a CTA of 384 threads, one per SM, persistent over tiles of 128
 // rows x BN weight rows:
 //   warp 0      TMA producer: 128 x 128 bytes of x and BN x 128 bytes of w per
-//               stage (128-byte swizzle)
+//               stage (128-byte swizzle); GATHER: the rows of x that a row
+//               table names, four per instruction
 //   warp 1      issues the MMAs of a block into one of 512 / BN TMEM buffers
-//   warp 2      allocates TMEM
-//   warp 2      also copies the block scales of the tile's rows and weights into
-//               shared memory, transposed, eight blocks at a time (read by the
-//               epilogue threads straight from global memory, a row each, they
-//               cost more than the MMAs: 32 cache lines per load)
+//   warp 2      allocates TMEM; copies the block scales of the tile's rows and
+//               weights into shared memory, transposed, in chunks of eight
+//               blocks that are up to 16 blocks ahead (their first touch can
+//               come from DRAM: 3500 cycles and more)
 //   warp 3      gate: waits for the sums of a block and lets the epilogue warps
 //               through a named barrier (a dozen warps polling shared-memory
 //               barriers slow down every barrier operation: a poll of a
 //               completed barrier went from 50 to 340 cycles)
 //   warps 4-11  promote: two warpgroups, BN / 2 columns each; at a tile's end
 //               they round, transpose through shared memory and store rows
-// A 128 x 256 tile needs 512 cycles of MMA per block; reading its 32768
-// accumulators takes 256 cycles of TMEM bandwidth and the FMAs 128 issue
-// slots per warp, so promotion hides behind the MMAs of the next block.
+// A block of a 128 x 256 tile is 512 cycles of MMA and 160 more until its end
+// is seen, 500 to 600 of promotion (TMEM read, scale, add) and about 150 of
+// hand-overs; with two TMEM buffers a block leaves every 850 to 1000 cycles.
+// That, and at 1000 W the clock (1.6 GHz), bounds large products: 8192 x 4096
+// x 14336 bf16 504 us, 1.91 PFLOP/s, tensor pipe 51% busy. Few rows are bound
+// by the weights' bytes: 8 experts of 4096 x 14336, 16 rows, 5.4 TB/s.
 //
 // SPLIT: few tiles. A cluster of S CTAs shares a tile, each takes a range of
 // blocks; the partial tiles meet in distributed shared memory and are added
 // in rank order, so no workspace is needed and the result does not depend on
-// timing.
+// timing. (64 rows, 4096 x 4096: 11.4 us with S = 4, 15.4 with one CTA per
+// tile; the cluster itself costs 3.5 us.)
 //
 // Every wait is bounded; when one runs out the CTA raises STATUS_TIMEOUT, lets
 // its copies and MMAs land, frees TMEM and returns.
@@ -715,13 +719,21 @@ int launch_gemm_f8(const F8Gemm &p, cudaStream_t s) {
     q.tiles_n = (int)nt;
     q.band = 16;
     if (nt * m128 > INT32_MAX / 2) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: too many tiles");
-    const int bn = nt * m256 >= sms ? 256 : 128;
+    // A block of a 128-column tile takes about 2/3 of the time of a 256-column
+    // one, so the wider tile wins unless the narrower saves a third of the
+    // rounds over the SMs or can be split (1024 rows, 4096 x 4096: 22.7 us at
+    // 256 columns, 33.7 at 128; 64 rows, 4096 x 14336: 21.4 and 17.2; 256 rows,
+    // 4096 x 4096: 20.9 and, in two, 15.3).
+    const int64_t cost256 = 3 * ((nt * m256 + sms - 1) / sms), cost128 = 2 * ((nt * m128 + sms - 1) / sms);
+    const int bn = cost256 <= cost128 ? 256 : 128;
     const int64_t tiles = nt * (bn == 256 ? m256 : m128);
     q.tiles_m = (int)(bn == 256 ? m256 : m128);
     q.max_tiles = (int)tiles;
     int split = 1;
     if (bn == 128)
         while (split < 8 && tiles * split * 2 <= sms && q.kb / (split * 2) >= 2) split *= 2;
+    // a block is 0.37 us, a cluster 3.5 us (64 rows, 1024 x 1024: REPLA us in one, 7.9 in four)
+    if (q.kb * (split - 1) < 12 * split) split = 1;
     CUtensorMap tm_w, tm_x;
     int rc = encode_tensor_map_3d_sw128(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, (uint64_t)p.K, (uint64_t)p.M,
                                         (uint64_t)n_exp, p.w_nb1, n_exp > 1 ? p.w_nb2 : p.w_nb1 * (uint64_t)p.M, F8B,

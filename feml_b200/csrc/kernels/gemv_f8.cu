@@ -222,7 +222,7 @@ int launch_gemv_f8(const F8Gemm &p, cudaStream_t s) {
     const bool few = tiles * 2 <= sm_count();
     const int warps = few || tiles >= 2 * sm_count() || kb < 16 ? 8 : 16;
     int splits = 1;
-    while (few && splits < 8 && tiles * splits * 2 <= sm_count() && kb >= 2 * splits * warps) splits *= 2;
+    while (few && splits < 8 && tiles * splits * 2 <= sm_count() && kb >= 4 * splits * warps) splits *= 2;
     if (tiles * splits > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: too many tiles");
     const int ctas = (int)(tiles * splits);
     if (p.out_type == FB_F32) return launch_w<float>(p, warps, ctas, splits, s);
