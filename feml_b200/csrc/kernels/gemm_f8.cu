@@ -396,7 +396,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                     __syncwarp();
                     if (GATHER) {
                         if (lane < boxes) tma_gather4(xs + lane * 4 * F8B, &tm_x, b * F8B, r[0], r[1], r[2], r[3], bar);
-                    } else if (lane < boxes) tma_load_2d(xs + lane * G_XBOX * F8B, &tm_x, b * F8B, tile.row0 + lane * G_XBOX, bar);
+                    } else if (lane < boxes) {
+                        tma_load_2d(xs + lane * G_XBOX * F8B, &tm_x, b * F8B, tile.row0 + lane * G_XBOX, bar);
+                    }
                 }
             }
             if (*abort_flag)  // let the copies in flight land before the CTA exits
@@ -510,25 +512,23 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                 // scales of the next block are read behind this block's loads
                 const float *sxc = &sx[c * G_SCB * G_SCP + row], *swc = &sw[c * G_SCB * 2 + grp * C::COLS / F8B];
                 if (j == 0) sc = sxc[0] * swc[0];
-                {
-                    tc_fence_after();
-                    const uint64_t sc2 = f2_pack(sc, sc);
-                    uint32_t v[2][16];
-                    tc_ld16(lanes + (uint32_t)(u * BN), v[0]);
-                    const int jn = j + 1 < G_SCB ? j + 1 : 0;
-                    sc = sxc[jn * G_SCP] * swc[jn * 2];
-                    tc_wait_ld();
+                tc_fence_after();
+                const uint64_t sc2 = f2_pack(sc, sc);
+                uint32_t v[2][16];
+                tc_ld16(lanes + (uint32_t)(u * BN), v[0]);
+                const int jn = j + 1 < G_SCB ? j + 1 : 0;
+                sc = sxc[jn * G_SCP] * swc[jn * 2];
+                tc_wait_ld();
 #pragma unroll
-                    for (int h = 0; h < C::COLS / 16; h++) {
-                        if (h + 1 < C::COLS / 16) tc_ld16(lanes + (uint32_t)(u * BN + (h + 1) * 16), v[(h + 1) & 1]);
+                for (int h = 0; h < C::COLS / 16; h++) {
+                    if (h + 1 < C::COLS / 16) tc_ld16(lanes + (uint32_t)(u * BN + (h + 1) * 16), v[(h + 1) & 1]);
 #pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            f2_fma_in_place(acc[h * 8 + i], f2_pack_bits(v[h & 1][2 * i], v[h & 1][2 * i + 1]), sc2);
-                        if (h + 1 < C::COLS / 16) tc_wait_ld();
-                        if (h + 2 == C::COLS / 16) {  // all of it is in registers
-                            tc_fence_before();
-                            buf_arrive(u);
-                        }
+                    for (int i = 0; i < 8; i++)
+                        f2_fma_in_place(acc[h * 8 + i], f2_pack_bits(v[h & 1][2 * i], v[h & 1][2 * i + 1]), sc2);
+                    if (h + 1 < C::COLS / 16) tc_wait_ld();
+                    if (h + 2 == C::COLS / 16) {  // all of it is in registers
+                        tc_fence_before();
+                        buf_arrive(u);
                     }
                 }
                 if (j == G_SCB - 1 || b == b1 - 1) {
@@ -732,7 +732,7 @@ int launch_gemm_f8(const F8Gemm &p, cudaStream_t s) {
     int split = 1;
     if (bn == 128)
         while (split < 8 && tiles * split * 2 <= sms && q.kb / (split * 2) >= 2) split *= 2;
-    // a block is 0.37 us, a cluster 3.5 us (64 rows, 1024 x 1024: REPLA us in one, 7.9 in four)
+    // a block is 0.37 us, a cluster 3.5 us (64 rows, 1024 x 1024: 6.4 us in one, 7.9 in four)
     if (q.kb * (split - 1) < 12 * split) split = 1;
     CUtensorMap tm_w, tm_x;
     int rc = encode_tensor_map_3d_sw128(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, (uint64_t)p.K, (uint64_t)p.M,

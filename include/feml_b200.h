@@ -545,7 +545,7 @@ int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, ui
  * whose source lies outside x becomes zeros; both set bit 1 of *status
  * (device int32, may be NULL), and so do groups that together have more rows
  * than groups which do not overlap can have (some rows are then left as they
- * were). At most 1024 experts. */
+ * were). At most 1024 experts; K is at least 1. */
 int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, const float *w_scale,
                                  uint64_t w_scale_nb1, uint64_t w_scale_nb2, int64_t n_experts, const void *x,
                                  uint64_t x_nb1, int64_t n_x, const float *x_scale, uint64_t x_scale_nb1,

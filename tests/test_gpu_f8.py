@@ -531,14 +531,16 @@ def test_other_stream_and_graph():
         w, ws = ops.quantize_f8(rand(g, m, k, scale=0.05), 128)
         x, r, gamma = rand(g, n, k), rand(g, n, k), 1 + 0.1 * rand(g, k)
         counts, offsets = tables([n])
+        back = torch.arange(n - 1, -1, -1, dtype=torch.int32, device="cuda")
 
         def layer():
             q, s, h = ops.rms_norm_f8(x, gamma, 1e-5, residual=r)
             y = ops.mul_mat_f8(w, ws, q, s)
             z = ops.mul_mat_f8_grouped(w[None], ws[None], q, s, counts, offsets)
+            z2 = ops.mul_mat_f8_grouped(w[None], ws[None], q, s, counts, offsets, rows=back)
             a, sa = ops.silu_mul_f8(y[:, :m // 2], z[:, m // 2:])
             b, sb = ops.quantize_f8(y)
-            return h, y, z, a.float(), sa, b.float(), sb
+            return h, y, z, z2, a.float(), sa, b.float(), sb
 
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
