@@ -212,6 +212,16 @@ def test_silu_mul_far_gates():
     check_f8(q, s, want, rel=64 * U)
 
 
+def test_silu_mul_subnormal_sigmoid():
+    """1 / (1 + exp(-gate)) is below the normal f32 range, the product with a large `up` is not."""
+    gate = torch.tensor([[-88.5, -88.0, -87.75, -87.5, -87.25, -87.0, -80.0, -60.0] * 16], device="cuda")
+    up = torch.full_like(gate, 3e38)
+    q, s = ops.silu_mul_f8(gate, up)
+    g = gate.double()
+    # the exponential as above; the reciprocal 2^-127 and below has 22 bits left, one unit of which is 2^-22
+    check_f8(q, s, g / (1 + torch.exp(-g)) * up.double(), rel=2 * U * (2 + 1.173 * 88.5 + 2 + 2 + 2))
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # products
 # ---------------------------------------------------------------------------------------------------------------
