@@ -45,6 +45,10 @@ __global__ void __launch_bounds__(A_THREADS) gemm_f8_any_kernel(const F8Gemm p) 
         __syncthreads();
         grp = s_grp;
         if (grp.expert < 0) return;
+        if (blockIdx.x == gridDim.x - 1) {  // a tile that groups which do not overlap never have
+            if (tid == 0) report_status(p.status, STATUS_BAD_ID);
+            return;
+        }
     } else {
         grp.rows = min(AB, p.N - grp.row0);
     }
@@ -122,7 +126,8 @@ __global__ void __launch_bounds__(A_THREADS) gemm_f8_any_kernel(const F8Gemm p) 
 }  // namespace
 
 int launch_gemm_f8_any(const F8Gemm &p, cudaStream_t s) {
-    // every group's last tile may be a partial one
+    // every group's last tile may be a partial one, which makes fewer tiles than
+    // this: the last index is left for groups that overlap
     const int64_t gx = ((int64_t)p.N + AB - 1) / AB + (p.g.counts ? p.g.n_experts : 0);
     const int64_t gy = ((int64_t)p.M + AB - 1) / AB;
     if (gy > 65535) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: %d rows of unaligned weights", p.M);

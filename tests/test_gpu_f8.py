@@ -478,6 +478,32 @@ def test_grouped_overlapping_tables_end():
     assert torch.all(buf[0] == 5.0) and torch.all(buf[n + 1] == 5.0) and torch.isfinite(buf).all()
 
 
+@pytest.mark.parametrize("k", [256, 253])
+def test_grouped_overlap_is_reported_for_any_alignment(k):
+    m, e, n = 70, 40, 300
+    w, ws, x, xs = operands(3, n, k, m, e)
+    c, o = tables([n] + [0] * (e - 1))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = ops.mul_mat_f8_grouped(w, ws, x, xs, c, o, status=status)
+    check_product(out, *product64(w[0], ws[0], x, xs), k)
+    assert int(status) == 0
+    ops.mul_mat_f8_grouped(w, ws, x, xs, torch.full_like(c, n), torch.zeros_like(o), out=out, status=status)
+    assert int(status) == 2 and torch.isfinite(out).all()
+
+
+def test_grouped_fullest_proper_tables_of_any_alignment():
+    """As many tiles as groups that do not overlap can have: none of them is refused."""
+    for counts in ([1], [64], [65], [1, 1, 1], [65, 65, 65], [64, 1, 64, 1], [63, 66, 128, 129]):
+        n, k, m = sum(counts), 37, 66
+        w, ws, x, xs = operands(4, n, k, m, len(counts))
+        c, o = tables(counts)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = ops.mul_mat_f8_grouped(w, ws, x, xs, c, o, status=status)
+        assert int(status) == 0
+        for e, (at, cnt) in enumerate(zip(o.tolist(), counts)):
+            check_product(out[at:at + cnt], *product64(w[e], ws[e], x[at:at + cnt], xs[at:at + cnt]), k)
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # as they are used
 # ---------------------------------------------------------------------------------------------------------------
