@@ -596,6 +596,51 @@ def test_other_stream_and_graph():
             assert torch.equal(a, b)
 
 
+def test_graph_behind_copies_and_joined_streams():
+    """Captured calls whose predecessors are copies, fills and the ends of other streams' work, then each other."""
+    g = gen(77)
+    n, k, m = 40, 512, 384
+    w, ws = ops.quantize_f8(rand(g, m, k, scale=0.05), 128)
+    src = [rand(g, n, k) for _ in range(3)]
+    x, r, z = (torch.empty(n, k, device="cuda") for _ in range(3))
+    gamma = 1 + 0.1 * rand(g, k)
+    host = torch.empty(n, m).pin_memory()
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def layer():
+        here = torch.cuda.current_stream()
+        x.copy_(src[0])
+        q0, s0 = ops.quantize_f8(x)  # behind a copy
+        z.zero_()
+        qz, sz = ops.quantize_f8(z)  # behind a fill
+        other.wait_stream(here)
+        with torch.cuda.stream(other):
+            r.copy_(src[1])
+            y1 = ops.mul_mat_f8(w, ws, q0, s0)
+        y0 = ops.mul_mat_f8(w, ws, qz, sz)
+        here.wait_stream(other)
+        q, s, h = ops.rms_norm_f8(x, gamma, 1e-5, residual=r)  # behind both streams
+        y = ops.mul_mat_f8(w, ws, q, s)
+        y1.add_(y)
+        host.copy_(y1, non_blocking=True)
+        qy, sy = ops.quantize_f8(y1)  # behind a copy to the host
+        return y0, y1, h, qy.float(), sy
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        want = [t.clone() for t in layer()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = layer()
+    for _ in range(3):
+        for t in (x, r, z, *got):
+            t.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(host, want[1].cpu())
+
+
 def test_two_streams_at_once():
     """Products on two streams at the same time share nothing."""
     sets = [operands(s, 30, 4096, 1024) for s in (1, 2)]
