@@ -641,6 +641,54 @@ def test_graph_behind_copies_and_joined_streams():
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(host, want[1].cpu())
 
 
+def far(t, pitch):
+    """A copy of the matrix (or planes) t, the first dimension `pitch` bytes apart."""
+    es = t.element_size()
+    buf = torch.empty((t.shape[0] - 1) * pitch + t[0].numel() * es, dtype=torch.uint8, device="cuda")
+    v = buf.view(t.dtype).as_strided(t.shape, (pitch // es, *t[0].stride()))
+    v.copy_(t)
+    return v
+
+
+def test_offsets_past_32_bits():
+    """Rows, scales and experts whose byte offsets pass 2^32: the same bits as operands of the same alignment in one
+    place give."""
+    g, k, m = gen(5), 512, 200
+    far3, far20 = (2 << 30) + 4096, (1 << 28) + 4096  # of 3 rows the last, of 20 rows the last four
+
+    x, r = rand(g, 3, k).bfloat16(), rand(g, 3, k).bfloat16()
+    gamma = 1 + 0.1 * rand(g, k)
+    for pitch in (far3, far3 + 2):  # the second is aligned to elements only
+        fx, fr, h = far(x, pitch), far(r, pitch), far(r, pitch)
+        near = far(x, 4096 + pitch - far3)  # (a row's sum of squares has an order per alignment)
+        out = [far(torch.zeros(3, k, dtype=F8, device="cuda"), pitch), far(torch.zeros(3, k // 128, device="cuda"), far3)]
+        for want, got in ((ops.quantize_f8(x), lambda: ops.quantize_f8(fx, out=out[0], scale=out[1])),
+                          (ops.silu_mul_f8(x, r), lambda: ops.silu_mul_f8(fx, fr, out=out[0], scale=out[1])),
+                          (ops.rms_norm_f8(near, gamma, 1e-5, residual=r)[:2],
+                           lambda: ops.rms_norm_f8(fx, gamma, 1e-5, residual=fr, residual_out=h, out=out[0], scale=out[1])[:2])):
+            for a, b in zip(got(), want):
+                assert torch.equal(a.float(), b.float())
+        assert torch.equal(h, x + r)
+        del fx, fr, h, out
+
+    w, ws, x, xs = operands(6, 20, k, m)
+    for n, pitch in ((3, far3), (20, far20), (20, far20 + 4)):  # GEMV, TMA tiles, any alignment
+        fx, fxs, big = far(x[:n], pitch), far(xs[:n], pitch), far(torch.zeros(n, m, device="cuda"), pitch)
+        want = ops.mul_mat_f8(far(w, 528 if pitch % 16 == 0 else 516), ws, x[:n], xs[:n])
+        got = ops.mul_mat_f8(far(w, 528 if pitch % 16 == 0 else 516), ws, fx, fxs, out=big)
+        assert torch.equal(got, want)
+        del fx, fxs, big, got
+    fw = far(w, 25 << 20)  # 200 rows
+    for n in (3, 20):
+        assert torch.equal(ops.mul_mat_f8(fw, ws, x[:n], xs[:n]), ops.mul_mat_f8(w, ws, x[:n], xs[:n]))
+    del fw
+
+    w, ws, x, xs = operands(7, 24, k, m, 3)
+    c, o = tables([4, 0, 20])
+    assert torch.equal(ops.mul_mat_f8_grouped(far(w, far3), far(ws, far3), x, xs, c, o),
+                       ops.mul_mat_f8_grouped(w, ws, x, xs, c, o))
+
+
 def test_two_streams_at_once():
     """Products on two streams at the same time share nothing."""
     sets = [operands(s, 30, 4096, 1024) for s in (1, 2)]
