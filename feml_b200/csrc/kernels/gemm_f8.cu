@@ -37,8 +37,11 @@
 // timing. (64 rows, 4096 x 4096: 11.4 us with S = 4, 15.4 with one CTA per
 // tile; the cluster itself costs 3.5 us.)
 //
-// Every wait is bounded; when one runs out the CTA raises STATUS_TIMEOUT, lets
-// its copies and MMAs land, frees TMEM and returns.
+// Every wait for another role's progress is an mbarrier wait with a limit, so
+// that a role that gives up leaves nobody behind; when one runs out the CTA
+// raises STATUS_TIMEOUT, lets its copies and MMAs land, frees TMEM and returns.
+// (TMEM buffers handed back through a named barrier, which has no limit: 32
+// and 64 rows, 4096 x 14336, 0.6 to 0.9 us less of 17.2, others no different.)
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -79,7 +82,7 @@ struct GCfg {
     static constexpr int OFF_SX = OFF_GRP + (G_MAX_E + 1) * 4 + 12;
     static constexpr int OFF_SW = OFF_SX + G_SCR * G_SCB * G_SCP * 4;
     static constexpr int OFF_BAR = OFF_SW + G_SCR * G_SCB * 2 * 4;
-    static constexpr int BYTES = OFF_BAR + (2 * NS + NB + 2 * G_SCR + 1) * 8 + 16 + 1024;
+    static constexpr int BYTES = OFF_BAR + (2 * NS + 2 * NB + 2 * G_SCR + 1) * 8 + 16 + 1024;
     static_assert(OFF_BAR % 8 == 0 && BYTES <= 232448, "shared memory");
     static_assert(GM * (BN + 4) * 4 <= NS * STAGE, "partial tile of a split");
 };
@@ -113,15 +116,9 @@ __device__ __forceinline__ void f2_fma_in_place(uint64_t &c, uint64_t a, uint64_
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
 }
 
-// A TMEM buffer is free again: the epilogue warps arrive, the MMA warp waits.
-__device__ __forceinline__ void buf_arrive(int u) {
-    asm volatile("bar.arrive %0, %1;" ::"r"(2 + u), "n"(32 * (G_EPI_WARPS + 1)) : "memory");
-}
-__device__ __forceinline__ void buf_wait(int u) {
-    asm volatile("bar.sync %0, %1;" ::"r"(2 + u), "n"(32 * (G_EPI_WARPS + 1)) : "memory");
-}
-
-// The gate warp and the epilogue warps meet once per block.
+// The gate warp and the epilogue warps meet once per block: the kernel's only
+// wait without a limit. Both sides walk every block of every tile, after an
+// abort too, so they pass it in the same number.
 __device__ __forceinline__ void gate_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(32 * (G_EPI_WARPS + 1)) : "memory");
 }
@@ -296,7 +293,8 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     uint64_t *full = reinterpret_cast<uint64_t *>(gbase + C::OFF_BAR);
     uint64_t *empty = full + C::NS;
     uint64_t *t_full = empty + C::NS;
-    uint64_t *s_full = t_full + C::NB;
+    uint64_t *t_empty = t_full + C::NB;
+    uint64_t *s_full = t_empty + C::NB;
     uint64_t *s_empty = s_full + G_SCR;
     uint64_t *drained = s_empty + G_SCR;
     float *sx = reinterpret_cast<float *>(gbase + C::OFF_SX);
@@ -315,7 +313,10 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < C::NB; i++) mbar_init(&t_full[i], 1);
+        for (int i = 0; i < C::NB; i++) {
+            mbar_init(&t_full[i], 1);
+            mbar_init(&t_empty[i], G_EPI_WARPS);
+        }
         for (int i = 0; i < G_SCR; i++) {
             mbar_init(&s_full[i], 32);
             mbar_init(&s_empty[i], G_EPI_WARPS);
@@ -416,9 +417,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                 if (g_tile(q, start, t, BN).expert < 0) break;
                 for (int b = b0; b < b1; b++, it++) {
                     const int s = it % C::NS, u = it % C::NB;
-                    ok = ok && tc_wait_all(&full[s], (it / C::NS) & 1, abort_flag);
-                    if (it >= C::NB) buf_wait(u);
-                    if (!ok) continue;  // (after an abort: the handshakes only)
+                    ok = ok && tc_wait_all(&full[s], (it / C::NS) & 1, abort_flag) &&
+                         tc_wait_all(&t_empty[u], ((it / C::NB) & 1) ^ 1, abort_flag);
+                    if (!ok) continue;
                     tc_fence_after();
                     const uint64_t xd = desc0 + (uint64_t)(s * (C::STAGE / 16)), wd = xd + C::X_STAGE / 16;
                     const uint32_t d = tmem + (uint32_t)(u * BN);
@@ -432,7 +433,6 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                 }
             }
             if (elect_one()) tc_commit(smem_u32(drained));  // every MMA issued here
-            for (int i = max(0, it - C::NB); i < it; i++) buf_wait(i % C::NB);
         } else if (warp == 2) {
             // ---- scales: G_SCB blocks of 128 rows at a time, eight lanes per row -------------
             const int j = lane & 7;
@@ -528,7 +528,8 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                     if (h + 1 < C::COLS / 16) tc_wait_ld();
                     if (h + 2 == C::COLS / 16) {  // all of it is in registers
                         tc_fence_before();
-                        buf_arrive(u);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&t_empty[u]);
                     }
                 }
                 if (j == G_SCB - 1 || b == b1 - 1) {
