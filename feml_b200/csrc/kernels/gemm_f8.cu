@@ -366,6 +366,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     const int t0 = (int)blockIdx.x / S, t_step = SPLIT ? 0x40000000 : (int)gridDim.x;
     const int b0 = SPLIT ? (int)((int64_t)q.kb * rank / S) : 0, b1 = SPLIT ? (int)((int64_t)q.kb * (rank + 1) / S) : q.kb;
 
+    int copied = 0;  // producer: stages that copies were issued for
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G_REGS_REST));
         if (warp == 0) {
@@ -402,8 +403,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                     }
                 }
             }
-            if (*abort_flag)  // let the copies in flight land before the CTA exits
-                for (int i = max(0, it - C::NS); i < it; i++) mbar_wait_bounded(&full[i % C::NS], (i / C::NS) & 1);
+            copied = it;
         } else if (warp == 1) {
             // ---- MMA issuer -----------------------------------------------------
             // (the whole warp walks the loop and one elected lane issues: with
@@ -563,6 +563,10 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         }
     }
     __syncthreads();
+    // whoever aborted, and whenever: no copy outlives the CTA
+    if (warp == 0 && *abort_flag)
+        for (int i = max(0, copied - C::NS); i < copied; i++) mbar_wait_bounded(&full[i % C::NS], (i / C::NS) & 1);
+    __syncwarp();
     if constexpr (SPLIT) {
         cluster_arrive();
         cluster_wait();

@@ -150,3 +150,10 @@ def test_the_kernel_has_no_unbounded_hand_over():
     text = source()
     assert "bar.arrive" not in text
     assert len(re.findall(r"bar\.sync", text)) == 1 and "bar.red" not in text
+
+
+def test_the_kernel_lands_its_copies_whoever_aborted():
+    """Behind the CTA's last barrier, where the abort flag is final."""
+    text = source()
+    last = text.index("__syncthreads();", text.index("store_rows<T, C::COLS>("))
+    assert "mbar_wait_bounded(&full[" in text[last:]
