@@ -39,7 +39,9 @@
 //
 // Every wait for another role's progress is an mbarrier wait with a limit, so
 // that a role that gives up leaves nobody behind; when one runs out the CTA
-// raises STATUS_TIMEOUT, lets its copies and MMAs land, frees TMEM and returns.
+// writes NaN to its tile and to those that it has not finished, raises
+// STATUS_TIMEOUT where the call has a status word, lets its copies and MMAs
+// land, frees TMEM and returns.
 // (TMEM buffers handed back through a named barrier, which has no limit: 32
 // and 64 rows, 4096 x 14336, 0.6 to 0.9 us less of 17.2, others no different.)
 #include <cuda.h>
@@ -556,7 +558,13 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                 const uint32_t bad = __ballot_sync(0xffffffffu, src < 0);
                 const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | p.y_nb1) & 15) == 0;
                 const int rows = tile.rows - r_first;
-                if (rows > 0 && !*abort_flag)
+                // (set before the gate lets the first block through that is not
+                // what it should be: where it is still clear the sums are right)
+                if (*abort_flag) {
+#pragma unroll
+                    for (int i = 0; i < C::COLS / 2; i++) acc[i] = 0x7fffffff7fffffffull;
+                }
+                if (rows > 0)
                     store_rows<T, C::COLS>(acc, stage, p.y + (uint64_t)(tile.row0 + r_first) * p.y_nb1, p.y_nb1, rows,
                                            tile.m0 + grp * C::COLS, p.M, bad, lane, wide);
             }
@@ -574,7 +582,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         int broken = 0;  // in any CTA of the cluster
         for (int i = 0; i < S; i++) broken |= (int)dsmem_ld4(dsmem_map(const_cast<const int *>(abort_flag), (uint32_t)i));
         static_assert(!SPLIT || BN == 128, "four columns per lane");
-        if (tile.expert >= 0 && !broken) {
+        if (tile.expert >= 0) {
             // rows rank, rank + S, ...: the S partial rows, all of them on the way
             // before the first is added (one after the other they cost 3 us),
             // in rank order
@@ -595,6 +603,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                         f[2] += __int_as_float(v[i].z);
                         f[3] += __int_as_float(v[i].w);
                     }
+                if (broken) f[0] = f[1] = f[2] = f[3] = __int_as_float(0x7fffffff);
                 T *o = reinterpret_cast<T *>(p.y + (uint64_t)(tile.row0 + r) * p.y_nb1) + m;
                 if (wide) {
                     if constexpr (sizeof(T) == 4)

@@ -390,7 +390,8 @@ def mul_mat_f8_grouped(w, w_scale, x, x_scale, counts, offsets, rows=None, n_sel
     int32 as moe_route gives them. -> [len(rows) or n, M]; rows of `out` in no
     group are left as they were (zeros when `out` is not given). `workspace`:
     uint8, mul_mat_f8_grouped_workspace bytes (allocated when needed). `status`:
-    int32 [1], bit 1 is set where a table points outside its range."""
+    int32 [1], bit 1 is set where a table points outside its range, bit 0 where
+    a wait inside the kernel ran out (the rows concerned are NaN)."""
     op = "mul_mat_f8_grouped"
     if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dim() != 3:
         raise FemlError("msg", f"{op}: w is not a 3-dimensional CUDA tensor")

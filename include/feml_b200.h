@@ -528,7 +528,9 @@ int feml_b200_silu_mul_f8(int32_t xtype, const void *gate, uint64_t gate_nb1, co
  * i*w_scale_nb1; x: e4m3, row n at x + n*x_nb1; x_scale row n at x_scale +
  * n*x_scale_nb1; dst row n at dst + n*dst_nb1. 16-byte aligned w and x with
  * strides that are multiples of 16 take the TMA kernels; any other alignment
- * works and is slower. No workspace, no allocation. */
+ * works and is slower. No workspace, no allocation. The call has no status
+ * word: should a wait inside the kernel run out (a GPU that no longer makes
+ * progress), the part of dst that it could not compute is NaN. */
 int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, uint64_t w_scale_nb1, const void *x,
                          uint64_t x_nb1, const float *x_scale, uint64_t x_scale_nb1, int32_t dst_type, void *dst,
                          uint64_t dst_nb1, int64_t K, int64_t M, int64_t N, void *stream);
@@ -545,7 +547,9 @@ int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, ui
  * whose source lies outside x becomes zeros; both set bit 1 of *status
  * (device int32, may be NULL), and so do groups that together have more rows
  * than groups which do not overlap can have (some rows are then left as they
- * were). At most 1024 experts; K is at least 1. */
+ * were). Bit 0 is set where a wait inside the kernel ran out, as in
+ * feml_b200_mul_mat_f8: the rows concerned are NaN. At most 1024 experts; K is
+ * at least 1. */
 int feml_b200_mul_mat_f8_grouped(const void *w, uint64_t w_nb1, uint64_t w_nb2, const float *w_scale,
                                  uint64_t w_scale_nb1, uint64_t w_scale_nb2, int64_t n_experts, const void *x,
                                  uint64_t x_nb1, int64_t n_x, const float *x_scale, uint64_t x_scale_nb1,

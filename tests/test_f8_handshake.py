@@ -157,3 +157,14 @@ def test_the_kernel_lands_its_copies_whoever_aborted():
     text = source()
     last = text.index("__syncthreads();", text.index("store_rows<T, C::COLS>("))
     assert "mbar_wait_bounded(&full[" in text[last:]
+
+
+def test_an_aborted_cta_writes_nan():
+    """Output that an aborted CTA could not compute is NaN, never what the buffer held: the stores are not skipped, and
+    both the plain and the cluster-split output look at the abort first."""
+    text = source()
+    assert "!*abort_flag" not in text and "!broken" not in text
+    plain = text[:text.index("store_rows<T, C::COLS>(")]
+    assert "acc[i] = 0x7fffffff7fffffffull" in plain[plain.rindex("if (*abort_flag)"):]
+    split = text[text.index("int broken = 0"):]
+    assert "if (broken) f[0] = f[1] = f[2] = f[3] = __int_as_float(0x7fffffff)" in split[:split.index("float4 *>(o)")]
