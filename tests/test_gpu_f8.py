@@ -222,6 +222,49 @@ def test_silu_mul_subnormal_sigmoid():
     check_f8(q, s, g / (1 + torch.exp(-g)) * up.double(), rel=2 * U * (2 + 1.173 * 88.5 + 2 + 2 + 2))
 
 
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("u", [3e38, -1e30, 1.0])
+@pytest.mark.parametrize("k", [1, 128, 136, 131])
+def test_silu_mul_gates_past_the_exponential(t, u, k):
+    """exp(-gate) is infinite in f32 below -88.7; the product with a large `up` is not 0 there. Every gate has blocks
+    of its own (single elements, 32-byte vectors, 16-byte ones), so their scales show it to f32's precision."""
+    gate = torch.cat([torch.linspace(-92.0, -86.0, 193), torch.linspace(-180.0, 0.0, 181)]).to(t).cuda()[:, None]
+    gate = gate.repeat(1, k)
+    up = torch.full_like(gate, u)
+    q, s = ops.silu_mul_f8(gate, up)
+    g = gate.double()
+    y = g * torch.exp(g) / (1 + torch.exp(g)) * up.double()
+    # each factor e^(g/2) is off by up to 2 + 1.173 * |g| / 2 units of 2^-23, the reciprocal by 1; four products, a sum
+    wq, ws = blocks64(y, 1)
+    rel = 2 * U * (4 + 1.173 * g[:, :1].abs() + 1 + 2 + 0.5)
+    assert torch.all((s.double() - ws).abs() <= ws * (rel + 2 * U))
+    check_f8(q, s, y, rel=2 * U * (4 + 1.173 * 180 + 3.5))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("k", [512, 515])
+def test_silu_mul_far_gates_among_near_ones(t, k):
+    """A lane with one far gate computes its near ones as the other lanes do, up to the last bits."""
+    g = gen(k)
+    gate = rand(g, 40, k, scale=2.0).to(t)
+    gate[::3, 7::31] = torch.tensor([-87.0, -87.5, -100.0, -500.0]).to(t).cuda().repeat(1, 99)[0, :gate[0, 7::31].numel()]
+    up = rand(g, 40, k, scale=3.0).to(t)
+    q, s = ops.silu_mul_f8(gate, up)
+    d = gate.double()
+    check_f8(q, s, d * torch.sigmoid(d) * up.double(), rel=2 * U * (4 + 1.173 * 20 + 3.5))
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_silu_mul_subnormal_gates(t):
+    """A gate below the normal range keeps its bits (f32 and bf16 have the same exponents)."""
+    least = 2.0 ** -149 if t == torch.float32 else 2.0 ** -133
+    gate = (torch.tensor([1.0, 3.0, 5.0, 127.0, -1.0, -7.0], dtype=torch.float64) * least).to(t).cuda()[:, None]
+    up = torch.full_like(gate, 2.0 ** 127)
+    q, s = ops.silu_mul_f8(gate, up)
+    # the reciprocal of 2 is off by one unit at most; two products that are not exact powers of two
+    check_f8(q, s, gate.double() / 2 * up.double(), rel=2 * U * 3)
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # products
 # ---------------------------------------------------------------------------------------------------------------
