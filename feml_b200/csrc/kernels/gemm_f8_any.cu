@@ -35,7 +35,9 @@ __global__ void __launch_bounds__(A_THREADS) gemm_f8_any_kernel(const F8Gemm p) 
     grid_dependency_wait();
     grid_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int m0 = blockIdx.y * AB;
+    const int64_t my = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;  // tile of weight rows
+    if (my * AB >= p.M) return;
+    const int m0 = (int)my * AB;
     F8Group grp{0, (int)blockIdx.x * AB, 0};
     if (p.g.counts) {
         if (warp == 0) {
@@ -129,9 +131,8 @@ int launch_gemm_f8_any(const F8Gemm &p, cudaStream_t s) {
     // every group's last tile may be a partial one, which makes fewer tiles than
     // this: the last index is left for groups that overlap
     const int64_t gx = ((int64_t)p.N + AB - 1) / AB + (p.g.counts ? p.g.n_experts : 0);
-    const int64_t gy = ((int64_t)p.M + AB - 1) / AB;
-    if (gy > 65535) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: %d rows of unaligned weights", p.M);
-    const dim3 grid((unsigned)gx, (unsigned)gy);
+    const int64_t tiles = ((int64_t)p.M + AB - 1) / AB, gz = (tiles + 65534) / 65535;  // grid.y has 16 bits
+    const dim3 grid((unsigned)gx, (unsigned)((tiles + gz - 1) / gz), (unsigned)gz);
     const char *what = "mul_mat_f8";
     if (p.out_type == FB_F32) return launch_early(what, gemm_f8_any_kernel<float>, grid, dim3(A_THREADS), 0, 1, s, p);
     if (p.out_type == FB_F16) return launch_early(what, gemm_f8_any_kernel<__half>, grid, dim3(A_THREADS), 0, 1, s, p);

@@ -330,6 +330,18 @@ def test_mul_mat_offset_pointers(n):
         assert torch.all(ob[:off] == 9.0)
 
 
+@pytest.mark.parametrize("m", [65535 * 64, 65535 * 64 + 1, 65535 * 64 * 2 + 70])
+def test_mul_mat_many_rows_of_any_alignment(m):
+    """More tiles of weight rows than one dimension of a grid has."""
+    w, ws, x, xs = operands(m % 1000, 2, 1, 300)
+    w = torch.cat([w.view(torch.uint8)] * (m // 300) + [w.view(torch.uint8)[:m % 300]]).view(F8)
+    ws = torch.rand(-(-m // 128), 1, generator=gen(1), device="cuda") + 0.5
+    buf = torch.full((2, m + 3), 5.0, dtype=torch.float16, device="cuda")
+    got = ops.mul_mat_f8(w, ws, x, xs, out=buf[:, :m])
+    check_product(got, *product64(w, ws, x, xs), 1)
+    assert torch.all(buf[:, m:] == 5.0)
+
+
 @pytest.mark.parametrize("n", [1, 12, 40, 140])
 def test_mul_mat_nan_and_range(n):
     """A NaN value or scale reaches its own rows and columns and no others; extreme scales keep their range."""
