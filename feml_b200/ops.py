@@ -414,10 +414,10 @@ def mul_mat_f8_grouped(w, w_scale, x, x_scale, counts, offsets, rows=None, n_sel
             need = mul_mat_f8_grouped_workspace(k, n_rows, e)
             if need:
                 workspace = torch.empty(need, dtype=torch.uint8, device=w.device)
-        else:
-            _f8_check(op, "workspace", workspace, torch.uint8, (workspace.numel(),), dev)
     elif n_selected != 1:
         raise FemlError("msg", f"{op}: n_selected = {n_selected} without rows")
+    if workspace is not None:
+        _f8_check(op, "workspace", workspace, torch.uint8, (workspace.numel() if isinstance(workspace, torch.Tensor) else 0,), dev)
     if status is not None:
         _f8_check(op, "status", status, torch.int32, (1,), dev)
     if out is None:

@@ -787,3 +787,15 @@ def test_refusals_on_the_gpu():
     for fn in bad:
         with pytest.raises(F.FemlError):
             fn()
+
+
+@pytest.mark.parametrize("gather", [False, True])
+def test_grouped_workspace_refusals(gather):
+    """A workspace is checked like every operand, whether the call would use it or not."""
+    w, ws, x, xs = operands(1, 40, 256, 130, 1)
+    c, o = tables([40])
+    rows = torch.arange(40, dtype=torch.int32, device="cuda") if gather else None
+    for bad in (b"bytes", torch.empty(20000, dtype=torch.uint8), torch.empty(5000, dtype=torch.int32, device="cuda"),
+                torch.empty(100, 200, dtype=torch.uint8, device="cuda"), torch.empty(40000, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(F.FemlError):
+            ops.mul_mat_f8_grouped(w, ws, x, xs, c, o, rows=rows, workspace=bad)
