@@ -158,6 +158,8 @@ SIGNATURES = [
                                      vp]),
     ("feml_b200_mul_mat_f8_grouped", c_int, [vp, c_u64, c_u64, vp, c_u64, c_u64, c_i64, vp, c_u64, c_i64, vp, c_u64, vp,
                                              vp, vp, c_i64, c_i32, vp, c_u64, c_i64, c_i64, c_i64, vp, c_u64, vp, vp]),
+    ("feml_b200_mul_mat_f8_plan", c_int, [c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(c_i32), ctypes.POINTER(c_i32),
+                                          ctypes.POINTER(c_i64), ctypes.POINTER(c_i32)]),
     ("feml_b200_mul_mat_f8_grouped_workspace", c_int, [c_i64, c_i64, c_i64, ctypes.POINTER(c_u64)]),
     ("feml_b200_buffer_from_host_ptr", c_int, [vp, vp, c_u64, c_u64, ctypes.POINTER(c_u32)]),
     ("feml_b200_gguf_open", c_int, [cp, ctypes.POINTER(vp)]),

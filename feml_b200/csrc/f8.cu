@@ -168,6 +168,25 @@ int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, ui
     return run_product(p, nullptr, 0, s);
 }
 
+int feml_b200_mul_mat_f8_plan(int64_t K, int64_t M, int64_t N, int64_t n_experts, int32_t *tile, int32_t *warps,
+                              int64_t *ctas, int32_t *split) {
+    const char *op = "mul_mat_f8_plan";
+    if (!tile || !warps || !ctas || !split) return set_error(FB_ERR_INVALID, "%s: null out", op);
+    FB_TRY(check_dims(op, K, M, N));
+    if (n_experts < 0 || n_experts > kMaxF8Experts)
+        return set_error(FB_ERR_UNSUPPORTED, "%s: %lld experts (0 to %lld)", op, (long long)n_experts, (long long)kMaxF8Experts);
+    *tile = *warps = *split = 0;
+    *ctas = 0;
+    if (K == 0 || M == 0 || N == 0) return FB_OK;
+    const fbk::F8Plan f = n_experts == 0 && N <= fbk::gemv_f8_max_rows() ? fbk::gemv_f8_plan(K, M)
+                                                                         : fbk::gemm_f8_plan(K, M, N, n_experts);
+    *tile = f.tile;
+    *warps = f.warps;
+    *ctas = f.ctas;
+    *split = f.split;
+    return FB_OK;
+}
+
 int feml_b200_mul_mat_f8_grouped_workspace(int64_t K, int64_t n_rows, int64_t n_experts, uint64_t *bytes) {
     const char *op = "mul_mat_f8_grouped_workspace";
     if (!bytes) return set_error(FB_ERR_INVALID, "%s: null out", op);

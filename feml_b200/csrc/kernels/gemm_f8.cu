@@ -720,34 +720,44 @@ int launch_gather_f8(F8Gemm &p, void *ws, cudaStream_t s) {
     return FB_OK;
 }
 
-int launch_gemm_f8(const F8Gemm &p, cudaStream_t s) {
-    const bool grouped = p.g.counts != nullptr, gather = grouped && p.g.rows;
+F8Plan gemm_f8_plan(int64_t K, int64_t M, int64_t N, int64_t n_experts) {
     const int sms = sm_count();
-    const int64_t n_exp = grouped ? p.g.n_experts : 1;
-    const int64_t m128 = (p.M + 127) / 128, m256 = (p.M + 255) / 256;
+    const int64_t kb = (K + F8B - 1) / F8B, m128 = (M + 127) / 128, m256 = (M + 255) / 256;
     // row tiles: exact, or the most that the groups can need
-    const int64_t nt = grouped ? std::min<int64_t>(p.N, p.N / GM + std::min<int64_t>(n_exp, p.N)) : (p.N + GM - 1) / GM;
-    GParams q{};
-    q.p = p;
-    q.kb = (p.K + F8B - 1) / F8B;
-    q.tiles_n = (int)nt;
-    q.band = 16;
-    if (nt * m128 > INT32_MAX / 2) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: too many tiles");
+    const int64_t nt = n_experts ? std::min<int64_t>(N, N / GM + std::min<int64_t>(n_experts, N)) : (N + GM - 1) / GM;
     // A block of a 128-column tile takes about 2/3 of the time of a 256-column
     // one, so the wider tile wins unless the narrower saves a third of the
     // rounds over the SMs or can be split (1024 rows, 4096 x 4096: 22.7 us at
     // 256 columns, 33.7 at 128; 64 rows, 4096 x 14336: 21.4 and 17.2; 256 rows,
     // 4096 x 4096: 20.9 and, in two, 15.3).
     const int64_t cost256 = 3 * ((nt * m256 + sms - 1) / sms), cost128 = 2 * ((nt * m128 + sms - 1) / sms);
-    const int bn = cost256 <= cost128 ? 256 : 128;
-    const int64_t tiles = nt * (bn == 256 ? m256 : m128);
-    q.tiles_m = (int)(bn == 256 ? m256 : m128);
-    q.max_tiles = (int)tiles;
-    int split = 1;
-    if (bn == 128)
-        while (split < 8 && tiles * split * 2 <= sms && q.kb / (split * 2) >= 2) split *= 2;
+    F8Plan f{};
+    f.tile = cost256 <= cost128 ? 256 : 128;
+    f.warps = G_THREADS / 32;
+    f.row_tiles = nt;
+    f.tiles = nt * (f.tile == 256 ? m256 : m128);
+    f.split = 1;
+    if (f.tile == 128)
+        while (f.split < 8 && f.tiles * f.split * 2 <= sms && kb / (f.split * 2) >= 2) f.split *= 2;
     // a block is 0.37 us, a cluster 3.5 us (64 rows, 1024 x 1024: 6.4 us in one, 7.9 in four)
-    if (q.kb * (split - 1) < 12 * split) split = 1;
+    if (kb * (f.split - 1) < 12 * f.split) f.split = 1;
+    f.ctas = f.split > 1 ? f.tiles * f.split : std::min<int64_t>(f.tiles, sms);
+    return f;
+}
+
+int launch_gemm_f8(const F8Gemm &p, cudaStream_t s) {
+    const bool grouped = p.g.counts != nullptr, gather = grouped && p.g.rows;
+    const int64_t n_exp = grouped ? p.g.n_experts : 1;
+    const F8Plan f = gemm_f8_plan(p.K, p.M, p.N, grouped ? n_exp : 0);
+    if (f.row_tiles * ((p.M + 127) / 128) > INT32_MAX / 2) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: too many tiles");
+    const int bn = f.tile, split = f.split, ctas = (int)f.ctas;
+    GParams q{};
+    q.p = p;
+    q.kb = (p.K + F8B - 1) / F8B;
+    q.tiles_n = (int)f.row_tiles;
+    q.band = 16;
+    q.tiles_m = (p.M + bn - 1) / bn;
+    q.max_tiles = (int)f.tiles;
     CUtensorMap tm_w, tm_x;
     int rc = encode_tensor_map_3d_sw128(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, (uint64_t)p.K, (uint64_t)p.M,
                                         (uint64_t)n_exp, p.w_nb1, n_exp > 1 ? p.w_nb2 : p.w_nb1 * (uint64_t)p.M, F8B,
@@ -756,8 +766,7 @@ int launch_gemm_f8(const F8Gemm &p, cudaStream_t s) {
     rc = encode_tensor_map_2d_sw128(&tm_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.x, (uint64_t)p.K,
                                     (uint64_t)(grouped ? p.g.n_x : p.N), p.x_nb1, F8B, gather ? 1 : G_XBOX);
     if (rc) return rc;
-    if (split > 1) return launch_g<128, true>(gather, tm_w, tm_x, q, (int)tiles * split, split, s);
-    const int ctas = (int)std::min<int64_t>(tiles, sms);
+    if (split > 1) return launch_g<128, true>(gather, tm_w, tm_x, q, ctas, split, s);
     if (bn == 256) return launch_g<256, false>(gather, tm_w, tm_x, q, ctas, 1, s);
     return launch_g<128, false>(gather, tm_w, tm_x, q, ctas, 1, s);
 }

@@ -211,20 +211,29 @@ int launch_w(const F8Gemm &p, int warps, int ctas, int splits, cudaStream_t s) {
 
 int gemv_f8_max_rows() { return 16; }
 
-int launch_gemv_f8(const F8Gemm &p, cudaStream_t s) {
-    const int64_t tiles = ((int64_t)p.M + V_ROWS - 1) / V_ROWS;
-    const int kb = (p.K + F8B - 1) / F8B;
+F8Plan gemv_f8_plan(int64_t K, int64_t M) {
+    const int64_t tiles = (M + V_ROWS - 1) / V_ROWS, kb = (K + F8B - 1) / F8B;
     // Two CTAs of eight warps per SM where there are tiles enough; one of
     // sixteen where there are not (one row, 4096 x 4096: 5.0 us, with eight
     // warps 6.7, with clusters of two 8.7); clusters of eight-warp CTAs only
     // where the tiles do not reach half of the SMs (16384 x 512: 5.4 us with
     // eight CTAs per tile, 17 with one).
     const bool few = tiles * 2 <= sm_count();
-    const int warps = few || tiles >= 2 * sm_count() || kb < 16 ? 8 : 16;
-    int splits = 1;
-    while (few && splits < 8 && tiles * splits * 2 <= sm_count() && kb >= 4 * splits * warps) splits *= 2;
-    if (tiles * splits > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: too many tiles");
-    const int ctas = (int)(tiles * splits);
+    F8Plan f{};
+    f.tile = V_ROWS;
+    f.warps = few || tiles >= 2 * sm_count() || kb < 16 ? 8 : 16;
+    f.row_tiles = 1;
+    f.tiles = tiles;
+    f.split = 1;
+    while (few && f.split < 8 && tiles * f.split * 2 <= sm_count() && kb >= 4 * f.split * f.warps) f.split *= 2;
+    f.ctas = tiles * f.split;
+    return f;
+}
+
+int launch_gemv_f8(const F8Gemm &p, cudaStream_t s) {
+    const F8Plan f = gemv_f8_plan(p.K, p.M);
+    if (f.ctas > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, "mul_mat_f8: too many tiles");
+    const int warps = f.warps, ctas = (int)f.ctas, splits = f.split;
     if (p.out_type == FB_F32) return launch_w<float>(p, warps, ctas, splits, s);
     if (p.out_type == FB_F16) return launch_w<__half>(p, warps, ctas, splits, s);
     return launch_w<__nv_bfloat16>(p, warps, ctas, splits, s);

@@ -293,13 +293,23 @@ struct F8Gemm {
     F8Groups g;
     int32_t *status;
 };
+// How a product's work is cut: weight rows per tile, warps per CTA, tiles of
+// output rows, tiles in all, CTAs of a cluster that share a tile, CTAs.
+struct F8Plan {
+    int tile, warps;
+    int64_t row_tiles, tiles;
+    int split;
+    int64_t ctas;
+};
 // gemm_f8_any.cu: any alignment.
 int launch_gemm_f8_any(const F8Gemm &p, cudaStream_t s);
 // gemv_f8.cu: up to gemv_f8_max_rows() rows of x, ungrouped (16-byte aligned rows).
 int gemv_f8_max_rows();
+F8Plan gemv_f8_plan(int64_t K, int64_t M);
 int launch_gemv_f8(const F8Gemm &p, cudaStream_t s);
 // gemm_f8.cu: tcgen05 tiles fed by TMA (16-byte aligned rows).
 bool gemm_f8_supported(const F8Gemm &p);
+F8Plan gemm_f8_plan(int64_t K, int64_t M, int64_t N, int64_t n_experts);  // 0 experts: ungrouped
 int launch_gemm_f8(const F8Gemm &p, cudaStream_t s);
 // Rows of x and their scales in the order of a grouped product's row table,
 // written to `ws` (gather_f8_bytes; 16-byte aligned); on return `p` reads

@@ -374,6 +374,16 @@ def mul_mat_f8(w, w_scale, x, x_scale, out=None, out_dtype=None):
     return out
 
 
+def mul_mat_f8_plan(K, M, N, n_experts=0):
+    """How a product of 16-byte aligned operands is cut -> (weight rows per
+    tile, warps per CTA, CTAs, CTAs that share a tile): mul_mat_f8 of N rows,
+    or with n_experts mul_mat_f8_grouped of N output rows."""
+    tile, warps, ctas, split = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int64(), ctypes.c_int32()
+    _check(_L.lib().feml_b200_mul_mat_f8_plan(K, M, N, n_experts, ctypes.byref(tile), ctypes.byref(warps),
+                                              ctypes.byref(ctas), ctypes.byref(split)))
+    return tile.value, warps.value, ctas.value, split.value
+
+
 def mul_mat_f8_grouped_workspace(K, n_rows, n_experts):
     """Workspace bytes for a product of n_rows rows with a row table."""
     v = ctypes.c_uint64()
@@ -433,4 +443,4 @@ def mul_mat_f8_grouped(w, w_scale, x, x_scale, counts, offsets, rows=None, n_sel
 
 __all__ = ["quantize", "mul_mat", "mul_mat_launches", "mul_mat_workspace", "mul_mat_noalloc", "mul_mat_noalloc_limit", "mul_mat_id", "mul_mat_id_workspace", "mul_mat_id_shard",
            "local_experts", "mul_mat_peer", "mul_mat_id_peer", "peer_wait", "moe_route",
-           "block_dots", "row_bytes", "quantize_f8", "rms_norm_f8", "silu_mul_f8", "mul_mat_f8", "mul_mat_f8_grouped", "mul_mat_f8_grouped_workspace", "FemlError"]
+           "block_dots", "row_bytes", "quantize_f8", "rms_norm_f8", "silu_mul_f8", "mul_mat_f8", "mul_mat_f8_plan", "mul_mat_f8_grouped", "mul_mat_f8_grouped_workspace", "FemlError"]

@@ -535,6 +535,15 @@ int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, ui
                          uint64_t x_nb1, const float *x_scale, uint64_t x_scale_nb1, int32_t dst_type, void *dst,
                          uint64_t dst_nb1, int64_t K, int64_t M, int64_t N, void *stream);
 
+/* How the current device cuts a product of 16-byte aligned operands (host
+ * only; 148 SMs without a GPU): weight rows per tile (32: the decode kernel of
+ * up to 16 rows; 128 or 256: tcgen05 tiles of 128 rows of x), warps per CTA,
+ * CTAs launched, and CTAs of a cluster that share a tile's sum over K.
+ * n_experts = 0: feml_b200_mul_mat_f8; above: feml_b200_mul_mat_f8_grouped
+ * with N rows of dst. All 0 where the call launches no product. */
+int feml_b200_mul_mat_f8_plan(int64_t K, int64_t M, int64_t N, int64_t n_experts, int32_t *tile, int32_t *warps,
+                              int64_t *ctas, int32_t *split);
+
 /* The same product for rows grouped by expert (ragged groups, known on the
  * device only): rows offsets[e] .. offsets[e] + counts[e] - 1 of dst are
  * multiplied with expert e's weights (w + e*w_nb2, w_scale + e*w_scale_nb2).

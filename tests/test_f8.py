@@ -91,3 +91,20 @@ def test_python_calls_refuse_host_tensors():
               lambda: ops.quantize_f8([1.0])):
         with pytest.raises(F.FemlError):
             f()
+
+
+def test_product_plans():
+    """The launch rules on the host (148 SMs without a GPU): rows per weight tile, warps, CTAs, CTAs per shared tile."""
+    plan = ops.mul_mat_f8_plan
+    assert plan(4096, 4096, 1) == (32, 16, 128, 1)      # one CTA of 16 warps per tile
+    assert plan(4096, 14336, 16) == (32, 8, 448, 1)     # two of eight per SM and more
+    assert plan(16384, 512, 8) == (32, 8, 128, 8)       # few tiles: clusters
+    assert plan(14336, 4096, 64) == (128, 12, 128, 4)   # few row tiles: clusters
+    assert plan(4096, 14336, 64) == (128, 12, 112, 1)
+    assert plan(4096, 14336, 8192) == (256, 12, 148, 1)
+    assert plan(4096, 14336, 16, 8) == (256, 12, 148, 1)
+    assert plan(4096, 200, 20, 2) == (128, 12, 32, 8)
+    assert plan(0, 5, 5) == plan(5, 0, 5) == plan(5, 5, 0) == (0, 0, 0, 0)
+    for bad in ((-1, 1, 1, 0), (1, 2 ** 31, 1, 0), (1, 1, 1, -1), (1, 1, 1, 1025)):
+        with pytest.raises(F.FemlError):
+            plan(*bad)
