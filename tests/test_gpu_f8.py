@@ -11,6 +11,7 @@ Tolerances (u = 2^-24, the half step of f32):
 """
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -136,6 +137,36 @@ def test_quantize_special_values(t, block_rows, k):
     assert torch.equal(torch.isnan(q.float()), spread)
     assert torch.all(q.float()[0:128, 0:128] == 0)
     assert torch.all(q.float()[128:256, 0:128] == -448)
+
+
+def test_scale_and_factor_are_correctly_rounded():
+    """scale = a / 448 and the factor 448 / a as IEEE division gives them: every mantissa of a, and a part of them at
+    every exponent that a block maximum can have. The factor shows through two neighbouring values of each row: the
+    last whose product with it is at most 17, halfway between the e4m3 values 16 and 18 (to even: 16), and the next."""
+    f = np.float32
+    m = (np.arange(1 << 23, dtype=np.uint32) | np.uint32(0x3F800000)).view(f)
+    r = f(448) / m
+    y = f(17) / r
+    for _ in range(4):
+        y = np.where(y * r > f(17), np.nextafter(y, f(0)), y)
+    for _ in range(4):
+        up = np.nextafter(y, f(1))
+        y = np.where(up * r <= f(17), up, y)
+    up = np.nextafter(y, f(1))
+    assert np.all(y * r <= f(17)) and np.all(up * r > f(17))
+    x = np.stack([m, y, up], 1)
+    s = m / f(448)
+    q = torch.tensor([448.0, 16.0, 18.0], device="cuda").to(F8).view(torch.uint8)
+
+    def same(x, s):
+        got, scale = ops.quantize_f8(torch.from_numpy(x).cuda())
+        assert torch.equal(scale[:, 0], torch.from_numpy(s).cuda())
+        assert torch.equal(got.view(torch.uint8), q.expand(len(x), 3))
+
+    same(x, s)
+    part = np.random.default_rng(1).integers(0, 1 << 23, 1 << 12)
+    for e in range(-100, 128):
+        same(np.ldexp(x[part], e), np.ldexp(s[part], e))
 
 
 @pytest.mark.parametrize("t", TYPES)
