@@ -247,6 +247,37 @@ def test_short_rows(n, k):
     check_product(ops.mul_mat_f8_grouped(w[None], ws[None], x, xs, c, o), *product64(w, ws, x, xs), k)
 
 
+def ends(q, fill):
+    """q [.., r, k] with rows 16-byte aligned and `fill` behind each row's end."""
+    k = q.shape[-1]
+    wide = torch.full((*q.shape[:-1], (k + 15) // 16 * 16 + 16), fill, dtype=torch.uint8, device="cuda")
+    wide[..., :k] = q.view(torch.uint8)
+    return wide.view(F8)[..., :k]
+
+
+@pytest.mark.parametrize("k", [5, 131, 1299, 2051])
+@pytest.mark.parametrize("n,m", [(1, 2500), (12, 200), (40, 200), (300, 300), (700, 3210)])
+def test_row_ends_inside_a_vector(n, m, k):
+    """Aligned rows whose length is no multiple of 16: the NaN bytes behind their ends count for nothing."""
+    w, ws, x, xs = operands(n + k, n, k, m)
+    got = ops.mul_mat_f8(ends(w, 0x7F), ws, ends(x, 0xFF), xs)
+    check_product(got, *product64(w, ws, x, xs), k)
+
+
+@pytest.mark.parametrize("k", [5, 1299, 2051])
+@pytest.mark.parametrize("work", ["none", "empty", "given"])
+def test_row_ends_inside_a_vector_grouped(k, work):
+    e, counts, m = 3, [50, 0, 71], 300
+    c, o = tables(counts)
+    w, ws, x, xs = operands(k, 40, k, m, e)
+    rows = torch.randint(0, 40, (121,), generator=gen(k), device="cuda", dtype=torch.int32)
+    need = ops.mul_mat_f8_grouped_workspace(k, 121, e)
+    room = {"none": None, "empty": torch.empty(0, dtype=torch.uint8, device="cuda"),
+            "given": torch.full((need,), 0x7F, dtype=torch.uint8, device="cuda")}[work]
+    got = ops.mul_mat_f8_grouped(ends(w, 0x7F), ws, ends(x, 0xFF), xs, c, o, rows=rows, workspace=room)
+    check_grouped(got, w, ws, x, xs, counts, o.tolist(), rows.long(), k)
+
+
 def test_captured_calls_of_every_kernel():
     """One graph with a wide, a split, a gathered and a decode product behind each other: the bits of eager calls."""
     k, m = 2064, 2500
