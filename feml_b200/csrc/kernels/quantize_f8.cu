@@ -112,10 +112,11 @@ __global__ void __launch_bounds__(kRowThreads, 2048 / kRowThreads) rows_f8_kerne
     const uint8_t *yr = SILU ? p.y + row * p.y_nb1 : nullptr;
     float f[N];
     uint32_t top = 0;
-    // (far gates: a lane that holds one reads its operands again, so that they
-    // need not be kept for it; with that and 32 registers, full occupancy: 35.7
-    // us, bf16 4096 x 11008. With 40 registers 37.3, with the form for any gate
-    // throughout 40.4.)
+    // (A lane that holds a far gate takes the form for any gate. That branch
+    // stands ahead of all arithmetic, and the launch bound holds the kernel to 32
+    // registers, full occupancy: bf16 4096 x 11008 35.4 us. With 40 registers
+    // 37.3, with the branch behind the near products 35.9, with the form for any
+    // gate throughout 40.4, without far gates 35.2.)
     if constexpr (W != 0) {
         const int64_t k = k0 + lane * N;  // k % N == 0 here: a vector lies inside the row or outside
         if (live && k < p.k) {
@@ -135,27 +136,28 @@ __global__ void __launch_bounds__(kRowThreads, 2048 / kRowThreads) rows_f8_kerne
             }
             bool far = false;
             if constexpr (SILU) far = silu_far<T>(v);
-#pragma unroll
-            for (int h = 0; h < N / V; h++) {
-                float x[V];
-                Vec<T>::get(v[h], x);
-                if constexpr (SILU) {
-                    float y[V];
-                    Vec<T>::get(u[h], y);
-#pragma unroll
-                    for (int i = 0; i < V; i++) x[i] = silu_mul_near(x[i], y[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < V; i++) f[h * V + i] = x[i];
-            }
-            if (far) {
+            if (SILU && far) {
 #pragma unroll
                 for (int h = 0; h < N / V; h++) {
                     float x[V], y[V];
-                    Vec<T>::get(ld_stream16(xr + k * sizeof(T) + h * 16), x);
-                    Vec<T>::get(ld_stream16(yr + k * sizeof(T) + h * 16), y);
+                    Vec<T>::get(v[h], x);
+                    Vec<T>::get(u[h], y);
 #pragma unroll
                     for (int i = 0; i < V; i++) f[h * V + i] = silu_mul_any(x[i], y[i]);
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < N / V; h++) {
+                    float x[V];
+                    Vec<T>::get(v[h], x);
+                    if constexpr (SILU) {
+                        float y[V];
+                        Vec<T>::get(u[h], y);
+#pragma unroll
+                        for (int i = 0; i < V; i++) x[i] = silu_mul_near(x[i], y[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < V; i++) f[h * V + i] = x[i];
                 }
             }
         } else {
