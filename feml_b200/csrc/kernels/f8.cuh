@@ -130,7 +130,7 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 // magnitude, both as IEEE division gives them, in a dozen instructions: a' =
 // m * 2^e with m in [1, 2), the quotients m / 448 and 448 / m by Newton's and
 // Markstein's corrections of an approximate reciprocal (q' = q + (n - q d) y
-// with fused multiply-adds; checked for all 2^23 m), then e added to or taken
+// with fused multiply-adds; tested for all 2^23 m), then e added to or taken
 // from their exponents, which stay normal for 2^-100 <= a' < 2^128. Two plain
 // divisions per block and lane took more issue slots than the rest of the row
 // kernels (bf16 8192 x 4096: 26.3 us).

@@ -27,14 +27,16 @@
 // A block of a 128 x 256 tile is 512 cycles of MMA and 160 more until its end
 // is seen, 500 to 600 of promotion (TMEM read, scale, add) and about 150 of
 // hand-overs; with two TMEM buffers a block leaves every 850 to 1000 cycles.
-// That, and at 1000 W the clock (1.6 GHz), bounds large products: 8192 x 4096
-// x 14336 bf16 504 us, 1.91 PFLOP/s, tensor pipe 51% busy. Few rows are bound
-// by the weights' bytes: 8 experts of 4096 x 14336, 16 rows, 5.4 TB/s.
+// That bounds large products: 8192 x 4096 x 14336 bf16 497 us in a run of a few
+// launches, 1.94 PFLOP/s, tensor pipe 51% busy; in a long run, where the 1000 W
+// cap takes the clock down to 1.6 GHz, 580 to 594 us. Few rows are bound by the
+// weights' bytes: 16 rows over experts of 4096 x 14336, five of them hit, 54 us,
+// 5.4 TB/s.
 //
 // SPLIT: few tiles. A cluster of S CTAs shares a tile, each takes a range of
 // blocks; the partial tiles meet in distributed shared memory and are added
 // in rank order, so no workspace is needed and the result does not depend on
-// timing. (64 rows, 4096 x 4096: 11.4 us with S = 4, 15.4 with one CTA per
+// timing. (64 rows, 4096 x 4096: 11.5 us with S = 4, 15.4 with one CTA per
 // tile; the cluster itself costs 3.5 us.)
 //
 // Every wait for another role's progress is an mbarrier wait with a limit, so
@@ -728,8 +730,12 @@ F8Plan gemm_f8_plan(int64_t K, int64_t M, int64_t N, int64_t n_experts) {
     // A block of a 128-column tile takes about 2/3 of the time of a 256-column
     // one, so the wider tile wins unless the narrower saves a third of the
     // rounds over the SMs or can be split (1024 rows, 4096 x 4096: 22.7 us at
-    // 256 columns, 33.7 at 128; 64 rows, 4096 x 14336: 21.4 and 17.2; 256 rows,
-    // 4096 x 4096: 20.9 and, in two, 15.3).
+    // 256 columns, 33.7 at 128; 64 rows, 4096 x 14336: 21.4 and 17.4; 256 rows,
+    // 4096 x 4096: 20.9 and, in two, 15.4). Grouped products follow the same
+    // rule from the most tiles that their groups can need (8 experts of 4096 x
+    // 14336, 16 rows: 54.9 us at 256 columns, 64.0 at 128; 1024 rows: 121.8,
+    // 165.0; 64 of 1408 x 2048, 18006 rows: 104, 128), though with few experts
+    // hit the narrower tile can be a little faster (two tokens: 51.6, 50.3).
     const int64_t cost256 = 3 * ((nt * m256 + sms - 1) / sms), cost128 = 2 * ((nt * m128 + sms - 1) / sms);
     F8Plan f{};
     f.tile = cost256 <= cost128 ? 256 : 128;
@@ -755,6 +761,9 @@ int launch_gemm_f8(const F8Gemm &p, cudaStream_t s) {
     q.p = p;
     q.kb = (p.K + F8B - 1) / F8B;
     q.tiles_n = (int)f.row_tiles;
+    // (16: 2048 rows, 4096 x 14336 129.9 us, 8192 rows 498; row tiles one by one
+    // 140.9 and 519; eight 131.6 and 504; 64 130.2 and 497, but 4096 rows of 4096 x
+    // 4096 81.7 instead of 77.6)
     q.band = 16;
     q.tiles_m = (p.M + bn - 1) / bn;
     q.max_tiles = (int)f.tiles;

@@ -2,7 +2,10 @@
 // not start on 16-byte boundaries cannot be fetched by TMA). 64 x 64 output
 // tiles, four warps of 32 x 32; one block of 128 values per step, staged
 // through shared memory with whatever alignment the rows have, multiplied
-// with m16n8k32 tensor-core instructions and scaled in f32.
+// with m16n8k32 tensor-core instructions and scaled in f32. Bound by those
+// (about 100 cycles each) and by staging, which nothing overlaps: 4096 x 4096
+// with one row 354 us, 512 rows 780 us, 2048 rows 2.1 ms, where aligned rows
+// take 5.5, 20 and 42 us.
 #include <cuda_runtime.h>
 
 #include "../host_common.h"

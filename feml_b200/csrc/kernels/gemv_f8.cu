@@ -13,8 +13,10 @@
 // order. Few weight rows: a cluster of S CTAs splits the blocks further and
 // adds its partial sums in rank order through distributed shared memory.
 // Bound by memory: each warp has two blocks (8 KB of weights) in flight (one
-// row, 4096 x 4096: 5.0 us, 3.3 TB/s; 4096 x 14336: 13.9 us, 4.2 TB/s; launch
-// and one memory round trip are 3 us of either).
+// row, 4096 x 4096: 5.3 us, 3.2 TB/s; 4096 x 14336: 13.9 us, 4.2 TB/s; launch
+// and one memory round trip are 3 us of either). Two groups of eight rows at
+// sixteen warps do not fit 128 registers: 92 bytes spilled with 16-byte loads,
+// 156 with 32-byte ones (16 rows, 4096 x 4096: 7.0 us).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -214,10 +216,15 @@ int gemv_f8_max_rows() { return 16; }
 F8Plan gemv_f8_plan(int64_t K, int64_t M) {
     const int64_t tiles = (M + V_ROWS - 1) / V_ROWS, kb = (K + F8B - 1) / F8B;
     // Two CTAs of eight warps per SM where there are tiles enough; one of
-    // sixteen where there are not (one row, 4096 x 4096: 5.0 us, with eight
-    // warps 6.7, with clusters of two 8.7); clusters of eight-warp CTAs only
-    // where the tiles do not reach half of the SMs (16384 x 512: 5.4 us with
-    // eight CTAs per tile, 17 with one).
+    // sixteen where there are not and every warp has a block (one row, 4096 x
+    // 4096: 5.3 us, with eight warps 6.7, with clusters of two 8.7; 2048 x 4096:
+    // 3.8 and 4.3; below 16 blocks, 1024 x 4096 with 16 rows, eight take 3.4 and
+    // sixteen 4.1; not borne out at 2048 x 8192, 6.8 and with eight 5.5, and at
+    // 16 rows of 2048 x 4096, 5.4 and 4.3); clusters of eight-warp CTAs only where
+    // the tiles do not reach half of the SMs (16384 x 512: 5.4 us with eight CTAs
+    // per tile, 17 with one) and every warp keeps two blocks or more (16 rows,
+    // 8192 x 512: 4.8 us, down to one block each 7.8; one row of 4096 x 512 would
+    // gain: 3.9 and 3.2).
     const bool few = tiles * 2 <= sm_count();
     F8Plan f{};
     f.tile = V_ROWS;

@@ -5,7 +5,8 @@
 // All of them are bound by memory: a few operations per byte, every value
 // read once and written once. The block maximum is taken of values that stay
 // in registers between the load and the store, so no operator makes a second
-// pass over its input.
+// pass over its input (but the norm of rows that are aligned to less than 16
+// bytes or too long for registers: norm_f8_any_kernel).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -346,7 +347,9 @@ __device__ __forceinline__ void st_wide(void *p, const uint4 (&v)[W / 16]) {
 }
 
 // The row in registers: NV vectors of W bytes per thread. WARP: a warp per
-// row (blockDim.y rows per CTA), else a CTA per row.
+// row (blockDim.y rows per CTA), else a CTA per row. (The bound of 1024 threads
+// holds NV = 4 at W = 32 to 64 registers; the 16-bit types spill 152 bytes
+// there. It takes rows of more than 32 KB, or 64 KB where rows are few.)
 template <typename T, int NV, bool WARP, int W>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8Params p) {
     constexpr int V = Vec<T>::N, H = W / 16, N = V * H, G = F8B / N;
@@ -460,7 +463,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_f8_kernel(const NormF8
 // Rows of any length and alignment: the sum of squares in one pass, the norm
 // in a second one that reads the stored sum (or x) again, a warp per block.
 // (A variant that held such rows in registers took 1.6 times as long at 4001 x
-// 4101 bf16: single elements need the occupancy more than the saved pass.)
+// 4101 bf16: single elements need the occupancy more than the saved pass.) With
+// a residual that takes 79 us, four times what the bytes take at the copy rate.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_f8_any_kernel(const NormF8Params p) {
     __shared__ float part[32];
@@ -534,7 +538,7 @@ int launch_norm_w(const NormF8Params &p, cudaStream_t s) {
         auto *fn = vecs <= 32 ? norm_f8_kernel<T, 1, true, W> : norm_f8_kernel<T, 2, true, W>;
         return launch_early(what, fn, dim3((unsigned)((p.rows + 7) / 8)), dim3(32, 8), 0, 1, s, p);
     }
-    const int most = p.rows <= 296 ? 1024 : 512;
+    const int most = p.rows <= 2 * sm_count() ? 1024 : 512;
     int nv = 1;
     while (nv < 4 && (vecs + nv - 1) / nv > most) nv *= 2;
     const int threads = (int)(((vecs + nv - 1) / nv + 31) / 32 * 32);

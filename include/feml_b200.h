@@ -493,8 +493,8 @@ int feml_b200_block_dots(int32_t wtype, const void *w, uint64_t w_nb1, const voi
  * FB_F16 or FB_BF16. Rows are contiguous, their strides (nb1, bytes) any
  * multiple of the element size that keeps rows apart. Sums, norms and
  * products are held in f32; dst is rounded once, to nearest even. Empty
- * operands (no rows, k = 0) are no error. Outputs must not overlap inputs,
- * except where said. */
+ * operands (no rows, k = 0) are no error (but K = 0 is one of the grouped
+ * product). Outputs must not overlap inputs, except where said. */
 #define FB_BF16 30
 
 /* rows x k values of x into the 8-bit form: q row r at q + r*q_nb1, and with
@@ -510,7 +510,9 @@ int feml_b200_quantize_f8(int32_t xtype, const void *x, uint64_t x_nb1, int64_t 
  * The norm is that of the stored sum, so the call gives the bits of an
  * addition followed by the norm. residual == NULL: h = x and sum is not
  * written. sum may be x or residual itself (exactly, same stride). weight: k
- * values of type wtype, the type of x or FB_F32. Relative of
+ * values of type wtype, the type of x or FB_F32. Rows, sum and weight aligned
+ * to 16 bytes are kept in registers; any other alignment (the weight's too)
+ * works and takes about four times as long. Relative of
  * feml_b200_graph_compute's rms_norm (feml-core/src/op.rs:26). */
 int feml_b200_rms_norm_f8(int32_t xtype, const void *x, uint64_t x_nb1, const void *residual, uint64_t residual_nb1,
                           void *sum, uint64_t sum_nb1, int32_t wtype, const void *weight, float eps, int64_t rows,
@@ -523,12 +525,12 @@ int feml_b200_silu_mul_f8(int32_t xtype, const void *gate, uint64_t gate_nb1, co
                           void *stream);
 
 /* mul_mat on the 8-bit form, ggml layout (dst row n = output column n):
- *   dst[n][m] = sum_b xs[n][b] * ws[m/128][b] * (sum_{k in b} x[n][k] * w[m][k])
+ *   dst[n][m] = sum_b (xs[n][b] * ws[m/128][b]) * (sum_{k in b} x[n][k] * w[m][k])
  * w: e4m3, row m at w + m*w_nb1; w_scale: block row i at w_scale +
  * i*w_scale_nb1; x: e4m3, row n at x + n*x_nb1; x_scale row n at x_scale +
  * n*x_scale_nb1; dst row n at dst + n*dst_nb1. 16-byte aligned w and x with
  * strides that are multiples of 16 take the TMA kernels; any other alignment
- * works and is slower. No workspace, no allocation. The call has no status
+ * works and is 40 times slower and more. No workspace, no allocation. The call has no status
  * word: should a wait inside the kernel run out (a GPU that no longer makes
  * progress), the part of dst that it could not compute is NaN. */
 int feml_b200_mul_mat_f8(const void *w, uint64_t w_nb1, const float *w_scale, uint64_t w_scale_nb1, const void *x,
