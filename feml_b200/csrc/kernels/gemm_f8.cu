@@ -29,7 +29,7 @@
 // hand-overs; with two TMEM buffers a block leaves every 850 to 1000 cycles.
 // That bounds large products: 8192 x 4096 x 14336 bf16 497 us in a run of a few
 // launches, 1.94 PFLOP/s, tensor pipe 51% busy; in a long run, where the 1000 W
-// cap takes the clock down to 1.6 GHz, 580 to 594 us. Few rows are bound by the
+// cap takes the clock down to 1.6 GHz, 580 to 596 us. Few rows are bound by the
 // weights' bytes: 16 rows over experts of 4096 x 14336, five of them hit, 54 us,
 // 5.4 TB/s.
 //
